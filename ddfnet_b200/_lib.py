@@ -18,6 +18,19 @@ MUL, ADD = 0, 1
 E_TOO_LARGE = -9
 VARIANT_AUTO, VARIANT_GENERIC, VARIANT_STREAM = 0, 1, 2
 
+NONE, SUM, MEAN = 0, 1, 2
+DISTILL_STATS, DISTILL_COUNTS = 8, 128
+
+
+class DistillArgs(ctypes.Structure):
+    """ddf_b200_distill_args"""
+    _fields_ = [("logits", ctypes.c_void_p), ("values", ctypes.c_void_p), ("indices", ctypes.c_void_p),
+                ("rest", ctypes.c_void_p), ("rows", ctypes.c_longlong), ("classes", ctypes.c_longlong),
+                ("row_stride", ctypes.c_longlong), ("k", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("values_dtype", ctypes.c_int), ("wide_indices", ctypes.c_int), ("reduction", ctypes.c_int),
+                ("temperature", ctypes.c_double)]
+
+
 # every symbol include/ddf_b200.h declares
 SYMBOLS = (
     "ddf_b200_version", "ddf_b200_strerror", "ddf_b200_forward", "ddf_b200_plan",
@@ -28,6 +41,7 @@ SYMBOLS = (
     "ddf_b200_frontend_tiles", "ddf_b200_pack_frontend", "ddf_b200_forward_waitlimit", "ddf_b200_band_waitlimit",
     "ddf_b200_forward_nhwc", "ddf_b200_nhwc_waitlimit", "ddf_b200_pool_nhwc_tiles", "ddf_b200_pool_nhwc",
     "ddf_b200_sfnorm", "ddf_b200_sfnorm_backward", "ddf_b200_maxpool_nhwc",
+    "ddf_b200_top_logits", "ddf_b200_distill_forward", "ddf_b200_distill_backward", "ddf_b200_distill_loss_grad",
     "ddf_b200_noop", "ddf_b200_rate_probe_bytes", "ddf_b200_rate_probe",
 )
 
@@ -70,6 +84,15 @@ def load() -> ctypes.CDLL:
         L.ddf_b200_pool_nhwc.argtypes = [vp, vp] + [i] * 5 + [vp]
         L.ddf_b200_maxpool_nhwc.restype = i
         L.ddf_b200_maxpool_nhwc.argtypes = [vp, vp] + [i] * 5 + [vp]
+        args = ctypes.POINTER(DistillArgs)
+        L.ddf_b200_top_logits.restype = i
+        L.ddf_b200_top_logits.argtypes = [vp] * 4 + [ll] * 3 + [i, ctypes.c_double, i, vp]
+        L.ddf_b200_distill_forward.restype = i
+        L.ddf_b200_distill_forward.argtypes = [args] + [vp] * 5
+        L.ddf_b200_distill_backward.restype = i
+        L.ddf_b200_distill_backward.argtypes = [args, vp, vp, vp, ll, vp, vp]
+        L.ddf_b200_distill_loss_grad.restype = i
+        L.ddf_b200_distill_loss_grad.argtypes = [args, vp, vp, vp, ctypes.c_double, vp, vp]
         L.ddf_b200_sfnorm.restype = i
         L.ddf_b200_sfnorm.argtypes = [vp, vp] + [i] * 5 + [ctypes.c_double, vp]
         L.ddf_b200_sfnorm_backward.restype = i

@@ -359,6 +359,7 @@ const char* ddf_b200_strerror(int status) {
         case DDF_B200_E_SCRATCH_LIMIT:
             return "ddf_b200: this problem needs more scratch than ddf_b200_backward_noalloc's "
                    "built-in 16 MiB array; use ddf_b200_backward with a caller-provided workspace";
+        case DDF_B200_E_ARGUMENT: return "ddf_b200: an argument is outside the range its declaration states";
         default: break;
     }
     if (status > 0) return cudaGetErrorString((cudaError_t)status);

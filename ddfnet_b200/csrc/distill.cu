@@ -1,0 +1,684 @@
+// Distillation from a teacher's top logits: loss and gradient of the student's logits.
+//
+// The classes of row n fall into K + 1 buckets: the K that the teacher lists (values t_k, classes i_k), and all
+// others together.  With a_k = t_k / T and a_rest = `rest` (the log of the others' sum of exp(t / T); -inf where
+// it is not given), b_k = s[i_k] / T and b_rest = log sum over the others of exp(s_j / T):
+//
+//   p = softmax(a),  q = softmax(b),  loss_n = T^2 sum_k p_k log(p_k / q_k)
+//   d loss_n / d s_j = T (q_k - p_k) for j = i_k;   T (q_rest - p_rest) exp(s_j / T - b_rest) for the others
+//
+// A class listed twice has the sum of its two probabilities; a class outside [0, V) is an empty entry; a row with
+// no entry, or no teacher mass, has loss 0 and gradient 0 and is not counted by the mean.
+//
+// Nothing cancels where student and teacher are near: with d = log(p / q) the summand is
+// p (d + expm1(-d)) = p d - p + q, never negative and of the same sum, and q - p = p expm1(-d).  A softmax's
+// largest entry is left out of its sum of exponentials, log1p of the others gives the logarithm.
+//
+// What bounds it: the logits' bytes, read once and, for the gradient, written once; 4 to 5 issue slots an
+// element besides.  Rows of up to 1024 elements stay in one warp's registers (distill_warp_kernel).  Longer ones
+// take a block, or a cluster of blocks whose slices fit shared memory (distill_block_kernel): loss and gradient
+// together then read the row once; across the cluster goes one (maximum, sum) pair a block.
+// A bitmap of the listed classes leaves them out of the running sum; their own values are gathered.
+#include <cooperative_groups.h>
+
+#include <atomic>
+
+#include "logits.cuh"
+
+namespace ddf {
+
+extern std::atomic<unsigned long long> g_launches;
+int device_facts(int* sm_count, int** fault, int* index);
+
+constexpr int kStats = 8;                     // floats a row between forward and backward
+constexpr int kSliceBytes = 64 * 1024;        // of a block's share of the row in shared memory: three blocks an SM
+constexpr int kWarpElements = 1024;           // a row (with what its first granule holds before it) in a warp
+constexpr int kCountBlocks = 128;
+enum { kLoss = 1, kGrad = 2 };
+
+struct DistillPlan {
+    const void *logits, *values, *indices;
+    const float* rest;
+    float *losses, *stats;
+    void* grad;
+    const float* upstream;
+    const int* counts;
+    long long stride, upstream_stride, rows;
+    int V, K, slices, per, n_counts;
+    int values_dtype, wide_indices;
+    float c, T, scale;
+};
+
+// One row's softmaxes over the buckets, in base 2:  log2 p_k = (a_k - ra) log2(e) - la,
+// log2 q_k = (s_k - m) c - top - lb.
+struct Row {
+    float ra, la, m, top, lb, rest_a, rest_b;  // rest_a = (a_rest - ra) log2(e), rest_b like (s_k - m) c
+    bool repeated;
+    __device__ __forceinline__ bool counted() const { return ra != neg_inf(); }
+};
+
+__device__ __forceinline__ float entry_value(const void* values, long long at, int dtype) {
+    if (dtype == DDF_B200_F32) return __ldg(reinterpret_cast<const float*>(values) + at);
+    if (dtype == DDF_B200_F16) return Elem<__half>::load(reinterpret_cast<const __half*>(values) + at);
+    return Elem<__nv_bfloat16>::load(reinterpret_cast<const __nv_bfloat16*>(values) + at);
+}
+// Class of an entry, -1 for an empty one.
+__device__ __forceinline__ int entry_class(const DistillPlan& p, long long at) {
+    const long long j = p.wide_indices ? __ldg(reinterpret_cast<const long long*>(p.indices) + at)
+                                       : (long long)__ldg(reinterpret_cast<const int*>(p.indices) + at);
+    return j >= 0 && j < p.V ? (int)j : -1;
+}
+
+// A softmax's logarithm of the sum, in base 2 and relative to its largest exponent: log2(1 + the others).
+// `sum` leaves out the entries equal to the largest, of which there are `ties`.
+__device__ __forceinline__ float log2_total(float sum, int ties) {
+    return log1pf(sum + (float)(ties - 1)) * kLog2e;
+}
+
+// The bucket softmaxes of a row from its entries in shared memory; called by whole warps, each for itself.
+__device__ __forceinline__ Row buckets(const float* a, const float* s, int K, float rest, const Online& others, float c) {
+    const int lane = threadIdx.x & 31;
+    float ra = rest, ms = neg_inf();
+    for (int k = lane; k < K; k += 32) {
+        ra = max_nan(ra, a[k]);
+        ms = max_nan(ms, s[k]);
+    }
+    Row r;
+    r.ra = warp_max_nan(ra);
+    r.m = max_nan(warp_max_nan(ms), others.m);
+    if (r.m == neg_inf()) r.m = 0.f;
+    const float base = r.ra == neg_inf() ? 0.f : r.ra;
+    r.rest_a = (rest - base) * kLog2e;
+    r.rest_b = others.s == 0.f ? neg_inf() : log2f(others.s) + (others.ref - r.m) * c;
+    float top = r.rest_b;
+    for (int k = lane; k < K; k += 32) top = max_nan(top, (s[k] - r.m) * c);
+    r.top = warp_max_nan(top);
+    if (r.top == neg_inf()) r.top = 0.f;
+    float sum_a = 0.f, sum_b = 0.f;
+    int ties_a = 0, ties_b = 0;
+    auto add = [&](float ea, float eb) {
+        if (ea == 0.f) ++ties_a; else sum_a += ex2(ea);
+        if (eb == 0.f) ++ties_b; else sum_b += ex2(eb);
+    };
+    for (int k = lane; k < K; k += 32) add((a[k] - base) * kLog2e, (s[k] - r.m) * c - r.top);
+    if (lane == 0) add(r.rest_a, r.rest_b - r.top);
+    // (without any tie all entries are -inf or one is NaN: the logarithm is then 0, or NaN)
+    ties_a = max(1, __reduce_add_sync(~0u, ties_a));
+    ties_b = max(1, __reduce_add_sync(~0u, ties_b));
+    r.la = log2_total(warp_sum(sum_a), ties_a);
+    r.lb = log2_total(warp_sum(sum_b), ties_b);
+    r.repeated = false;
+    return r;
+}
+
+// p log(p/q) - p + q of a bucket, and q - p, from the exponents log2 p and log2 q.
+__device__ __forceinline__ float term(float lp, float lq) {
+    const float p = ex2(lp), d = kLn2 * (lp - lq);
+    return p == 0.f ? ex2(lq) : p * (d + expm1f(-d));
+}
+__device__ __forceinline__ float q_minus_p(float lp, float lq) {
+    const float p = ex2(lp);
+    return p == 0.f ? ex2(lq) : p * expm1f(kLn2 * (lq - lp));
+}
+__device__ __forceinline__ float log2_p(const Row& r, float a) { return (a - r.ra) * kLog2e - r.la; }
+__device__ __forceinline__ float log2_q(const Row& r, float s, float c) { return (s - r.m) * c - r.top - r.lb; }
+
+// One warp: the row's loss.
+__device__ __forceinline__ float row_loss(const Row& r, const float* a, const float* s, int K, float c, float T) {
+    if (!r.counted()) return 0.f;
+    const int lane = threadIdx.x & 31;
+    float sum = lane == 0 ? term(r.rest_a - r.la, r.rest_b - r.top - r.lb) : 0.f;
+    for (int k = lane; k < K; k += 32) sum += term(log2_p(r, a[k]), log2_q(r, s[k], c));
+    return warp_sum(sum) * T * T;
+}
+
+__device__ __forceinline__ void put_stats(float* to, const Row& r) {
+    reinterpret_cast<float4*>(to)[0] = make_float4(r.ra, r.la, r.m, r.top);
+    reinterpret_cast<float4*>(to)[1] = make_float4(r.lb, r.rest_b, r.repeated ? 1.f : 0.f, 0.f);
+}
+__device__ __forceinline__ Row get_stats(const float* from, float rest) {
+    const float4 u = __ldg(reinterpret_cast<const float4*>(from)), v = __ldg(reinterpret_cast<const float4*>(from) + 1);
+    Row r;
+    r.ra = u.x; r.la = u.y; r.m = u.z; r.top = u.w;
+    r.lb = v.x; r.rest_b = v.y;
+    r.repeated = v.z != 0.f;
+    r.rest_a = (rest - (u.x == neg_inf() ? 0.f : u.x)) * kLog2e;
+    return r;
+}
+
+// Classes that are listed twice: the first entry takes the sum, the others become empty.  Every thread of the group
+// (`sync` is its barrier) handles the entries k = first, first + step, ...
+template <typename Sync>
+__device__ __noinline__ void merge_repeated(int* cls, float* a, float* s, int K, int first, int step, Sync sync) {
+    float sum[kMaxTop / 32];
+    uint32_t drop = 0;
+    int n = 0;
+    for (int k = first; k < K; k += step, ++n) {
+        const int j = cls[k];
+        if (j < 0) continue;
+        float m = neg_inf();
+        bool earlier = false;
+        for (int i = 0; i < K; ++i)
+            if (cls[i] == j) {
+                earlier |= i < k;
+                m = max_nan(m, a[i]);
+            }
+        float t = 0.f;
+        if (m != neg_inf())
+            for (int i = 0; i < K; ++i)
+                if (cls[i] == j) t += expf(a[i] - m);
+        sum[n] = m == neg_inf() ? m : m + logf(t);
+        if (earlier) drop |= 1u << n;
+    }
+    sync();
+    n = 0;
+    for (int k = first; k < K; k += step, ++n) {
+        if (cls[k] < 0) continue;
+        a[k] = sum[n];
+        if (drop >> n & 1u) {
+            cls[k] = -1;
+            a[k] = s[k] = neg_inf();
+        }
+    }
+    sync();
+}
+
+// Factor of the row's gradient: upstream, the loss scale and the mean's count, times T.  Whole warps.
+__device__ __forceinline__ float grad_factor(const DistillPlan& p, long long row) {
+    float g = p.scale * p.T;
+    if (p.upstream) g *= __ldg(p.upstream + row * p.upstream_stride);
+    if (p.counts) {
+        int n = 0;
+        for (int i = threadIdx.x & 31; i < p.n_counts; i += 32) n += __ldg(p.counts + i);
+        n = __reduce_add_sync(~0u, n);
+        g /= (float)max(n, 1);
+    }
+    return g;
+}
+
+// What the gradient of the others needs: g = factor * 2^((x - m) c - shift).
+struct Others {
+    float m, shift, factor;
+};
+__device__ __forceinline__ Others others_of(const Row& r, float g) {
+    Others o;
+    o.m = r.m;
+    o.shift = r.rest_b;
+    o.factor = g * q_minus_p(r.rest_a - r.la, r.rest_b - r.top - r.lb);
+    if (r.rest_b == neg_inf()) o.shift = o.factor = 0.f;  // no class has a share: all gradients are 0
+    return o;
+}
+template <int N> __device__ __forceinline__ void others_grad(const Others& o, float c, float (&x)[N]) {
+    const unsigned long long m2 = f2_pack(-o.m, -o.m), c2 = f2_pack(c, c), s2 = f2_pack(-o.shift, -o.shift);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        float a, b;
+        f2_unpack(f2_fma(f2_add(f2_pack(x[i], x[i + 1]), m2), c2, s2), a, b);
+        x[i] = o.factor * ex2(a);
+        x[i + 1] = o.factor * ex2(b);
+    }
+}
+
+// Stores granule g of a run's gradient.  `even`: the output's granules lie as the input's do.
+template <typename T>
+__device__ __forceinline__ void store_granule(const Run<T>& run, T* out, int g, bool even, const float (&x)[Granule<T>::N]) {
+    constexpr int N = Granule<T>::N;
+    const int e0 = g * N - run.phase;
+    if (even && e0 >= 0 && e0 + N <= run.len) {
+        const uint4 v = Granule<T>::put(x);
+        asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(out + e0), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (e0 + i >= 0 && e0 + i < run.len) Elem<T>::store(out + e0 + i, x[i]);
+    }
+}
+
+template <typename T> __device__ __forceinline__ float largest(const float (&x)[Granule<T>::N]) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < Granule<T>::N; ++i) m = max_nan(m, x[i]);
+    return m;
+}
+template <typename T> __device__ __forceinline__ void mask(float (&x)[Granule<T>::N], uint32_t bits) {
+#pragma unroll
+    for (int i = 0; i < Granule<T>::N; ++i)
+        if (bits >> i & 1u) x[i] = neg_inf();
+}
+
+// ------------------------------------------------------------------ a row in a warp
+constexpr int kRowWarps = 4;
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(32 * kRowWarps) distill_warp_kernel(const __grid_constant__ DistillPlan p) {
+    constexpr int N = Granule<T>::N;
+    constexpr int G = kWarpElements / N / 32;  // granules a lane
+    extern __shared__ __align__(16) unsigned char raw_shared[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long row = (long long)blockIdx.x * kRowWarps + warp;
+    if (row >= p.rows) return;
+    const int K = p.K;
+    uint32_t* bits = reinterpret_cast<uint32_t*>(raw_shared) + warp * (32 + 3 * K);
+    int* cls = reinterpret_cast<int*>(bits + 32);
+    float* a = reinterpret_cast<float*>(cls + K);
+    float* s = a + K;
+    const T* x = reinterpret_cast<const T*>(p.logits) + row * p.stride;
+    const Run<T> run(x, p.V);
+
+    uint4 raw[G];
+#pragma unroll
+    for (int u = 0; u < G; ++u)
+        if (lane + u * 32 < run.granules) raw[u] = run.load(lane + u * 32);
+    bits[lane] = 0;
+    __syncwarp();
+    bool twice = false;
+    for (int k = lane; k < K; k += 32) {
+        const int j = entry_class(p, row * K + k);
+        cls[k] = j;
+        a[k] = j < 0 ? neg_inf() : entry_value(p.values, row * K + k, p.values_dtype) / p.T;
+        s[k] = j < 0 ? neg_inf() : Elem<T>::load(x + j);
+        if (j >= 0) {
+            const uint32_t at = (uint32_t)(j + run.phase), bit = 1u << (at & 31u);
+            twice |= (atomicOr(bits + (at >> 5), bit) & bit) != 0;
+        }
+    }
+    const bool repeated = __any_sync(~0u, twice);
+    __syncwarp();
+    if (repeated) merge_repeated(cls, a, s, K, lane, 32, [] { __syncwarp(); });
+    bool any = false;
+    for (int k = lane; k < K; k += 32) any |= cls[k] >= 0;
+    any = __any_sync(~0u, any);
+    const float rest = any && p.rest ? __ldg(p.rest + row) : neg_inf();
+
+    Row r;
+    if constexpr (MODE & kLoss) {
+        Online others = Online::none();
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+            const int g = lane + u * 32;
+            if (g >= run.granules) break;
+            float v[N];
+            Granule<T>::get(raw[u], v);
+            const uint32_t out = (bits[g * N >> 5] >> (g * N & 31) & ((1u << N) - 1u)) | run.outside(g);
+            if (out) mask<T>(v, out);
+            others.add(v, largest<T>(v), p.c);
+        }
+        others = warp_merge(others, p.c);
+        r = buckets(a, s, K, rest, others, p.c);
+        r.repeated = repeated;
+        const float loss = row_loss(r, a, s, K, p.c, p.T);
+        if (lane == 0) {
+            p.losses[row] = loss;
+            if (p.stats) put_stats(p.stats + row * kStats, r);
+        }
+    } else {
+        r = get_stats(p.stats + row * kStats, rest);
+    }
+    if constexpr (MODE & kGrad) {
+        T* out = reinterpret_cast<T*>(p.grad) + row * p.V;
+        const bool even = (reinterpret_cast<unsigned long long>(out) & 15ull) == (reinterpret_cast<unsigned long long>(x) & 15ull);
+        const float g = grad_factor(p, row);
+        const Others o = others_of(r, g);
+        const bool counted = r.counted();
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+            const int i = lane + u * 32;
+            if (i >= run.granules) break;
+            float v[N];
+            Granule<T>::get(raw[u], v);
+            others_grad(o, p.c, v);
+            if (!counted) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] = 0.f;
+            }
+            store_granule(run, out, i, even, v);
+        }
+        __syncwarp();
+        if (counted)
+            for (int k = lane; k < K; k += 32)
+                if (cls[k] >= 0) Elem<T>::store(out + cls[k], g * q_minus_p(log2_p(r, a[k]), log2_q(r, s[k], p.c)));
+    }
+}
+
+// ------------------------------------------------------------------ a row in a block or a cluster
+constexpr int kRowThreads = 256;
+
+template <typename T, int MODE, bool RESIDENT>
+__global__ void __launch_bounds__(kRowThreads) distill_block_kernel(const __grid_constant__ DistillPlan p) {
+    constexpr int N = Granule<T>::N;
+    constexpr int NT = kRowThreads, UNROLL = 4;
+    extern __shared__ __align__(16) unsigned char raw_shared[];
+    __shared__ __align__(16) int cls[kMaxTop];
+    __shared__ float a[kMaxTop], s[kMaxTop];
+    __shared__ Online room[NT / 32], peers[8];
+    const int tid = threadIdx.x;
+    const int K = p.K;
+    const long long row = blockIdx.x / (unsigned)p.slices;
+    const int rank = (int)(blockIdx.x % (unsigned)p.slices);
+    const int v0 = rank * p.per;
+    const T* x = reinterpret_cast<const T*>(p.logits) + row * p.stride;
+    const Run<T> run(x + v0, min(p.per, p.V - v0));
+    uint4* copy = reinterpret_cast<uint4*>(raw_shared);
+    uint32_t* bits = reinterpret_cast<uint32_t*>(raw_shared + (RESIDENT ? (size_t)run.granules * 16 : 0));
+
+    if constexpr ((MODE & kLoss) != 0) {
+        if (p.slices > 1) cooperative_groups::this_cluster().barrier_arrive();
+        for (int i = tid; i < (run.granules * N + 31) / 32; i += NT) bits[i] = 0;
+    }
+    int mine = -1;
+    if (tid < K) {
+        mine = entry_class(p, row * K + tid);
+        cls[tid] = mine;
+        a[tid] = mine < 0 ? neg_inf() : entry_value(p.values, row * K + tid, p.values_dtype) / p.T;
+        s[tid] = mine < 0 ? neg_inf() : Elem<T>::load(x + mine);
+    }
+    const bool any = __syncthreads_or(mine >= 0);
+    const float rest = any && p.rest ? __ldg(p.rest + row) : neg_inf();
+    Row r;
+    bool repeated;
+    if constexpr ((MODE & kLoss) != 0) {
+        bool twice = false;
+        if (mine >= 0) {
+            if (mine >= v0 && mine < v0 + run.len) {
+                const uint32_t at = (uint32_t)(mine - v0 + run.phase);
+                atomicOr(bits + (at >> 5), 1u << (at & 31u));
+            }
+            for (int i = 0; i < tid; ++i) twice |= cls[i] == mine;
+        }
+        if (tid == 0) atomicOr(bits, run.outside(0));
+        if (tid == 1) atomicOr(bits + ((run.granules - 1) * N >> 5), run.outside(run.granules - 1) << ((run.granules - 1) * N & 31));
+        repeated = __syncthreads_or(twice);
+    } else {
+        r = get_stats(p.stats + row * kStats, rest);
+        repeated = r.repeated;
+    }
+    if (repeated) {
+        merge_repeated(cls, a, s, K, tid, NT, [] { __syncthreads(); });
+        if (tid < K) mine = cls[tid];
+    }
+
+    if constexpr ((MODE & kLoss) != 0) {
+        Online others = Online::none();
+        for (int g0 = tid; g0 < run.granules; g0 += NT * UNROLL) {
+            uint4 raw[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u)
+                if (g0 + u * NT < run.granules) raw[u] = run.load(g0 + u * NT);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int g = g0 + u * NT;
+                if (g >= run.granules) break;
+                if constexpr (RESIDENT) copy[g] = raw[u];
+                float v[N];
+                Granule<T>::get(raw[u], v);
+                const uint32_t out = bits[g * N >> 5] >> (g * N & 31) & ((1u << N) - 1u);
+                if (out) mask<T>(v, out);
+                others.add(v, largest<T>(v), p.c);
+            }
+        }
+        others = block_merge<NT / 32>(others, p.c, room);
+        if (p.slices > 1) {
+            auto cluster = cooperative_groups::this_cluster();
+            cluster.barrier_wait();  // every block of the cluster runs
+            if (tid < p.slices) *cluster.map_shared_rank(&peers[rank], tid) = others;
+            cluster.sync();
+            others = Online::none();
+            for (int i = 0; i < p.slices; ++i) others.merge(peers[i], p.c);
+        }
+        r = buckets(a, s, K, rest, others, p.c);
+        r.repeated = repeated;
+        if (rank == 0 && tid < 32) {
+            const float loss = row_loss(r, a, s, K, p.c, p.T);
+            if (tid == 0) {
+                p.losses[row] = loss;
+                if (p.stats) put_stats(p.stats + row * kStats, r);
+            }
+        }
+    }
+    if constexpr ((MODE & kGrad) != 0) {
+        T* out = reinterpret_cast<T*>(p.grad) + row * p.V;
+        const bool even = (reinterpret_cast<unsigned long long>(out + v0) & 15ull) == (reinterpret_cast<unsigned long long>(x + v0) & 15ull);
+        const float f = grad_factor(p, row);
+        const Others o = others_of(r, f);
+        const bool counted = r.counted();
+        for (int g0 = tid; g0 < run.granules; g0 += NT * UNROLL) {
+            uint4 raw[UNROLL];
+            if constexpr (!RESIDENT) {
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u)
+                    if (g0 + u * NT < run.granules) raw[u] = run.load(g0 + u * NT);
+            }
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int g = g0 + u * NT;
+                if (g >= run.granules) break;
+                float v[N];
+                Granule<T>::get(RESIDENT ? copy[g] : raw[u], v);
+                others_grad(o, p.c, v);
+                if (!counted) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) v[e] = 0.f;
+                }
+                store_granule(run, out + v0, g, even, v);
+            }
+        }
+        __syncthreads();  // the listed classes' gradients go over what the loop has put there
+        if (counted && mine >= v0 && mine < v0 + run.len)
+            Elem<T>::store(out + mine, f * q_minus_p(log2_p(r, a[tid]), log2_q(r, s[tid], p.c)));
+    }
+}
+
+// ------------------------------------------------------------------ counts and sums
+// Rows that count: some entry, and some teacher mass.  One partial count a block.
+template <int THREADS> __global__ void __launch_bounds__(THREADS) distill_count_kernel(const __grid_constant__ DistillPlan p, int* counts) {
+    __shared__ int warps[THREADS / 32];
+    const int lane = threadIdx.x & 31;
+    const long long step = (long long)gridDim.x * (THREADS / 32);
+    int n = 0;
+    for (long long row = (long long)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); row < p.rows; row += step) {
+        bool some = false;
+        for (int k = lane; k < p.K; k += 32)
+            if (entry_class(p, row * p.K + k) >= 0)
+                some |= entry_value(p.values, row * p.K + k, p.values_dtype) != neg_inf() || (p.rest && __ldg(p.rest + row) != neg_inf());
+        n += __any_sync(~0u, some);
+    }
+    if (lane == 0) warps[threadIdx.x >> 5] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int all = 0;
+        for (int w = 0; w < THREADS / 32; ++w) all += warps[w];
+        counts[blockIdx.x] = all;
+    }
+}
+
+// loss[0] = sum of the rows' losses, in one order, over their number where `mean`; count[0] = that number.
+constexpr int kSumThreads = 1024;
+__global__ void __launch_bounds__(kSumThreads) distill_sum_kernel(const float* losses, const float* stats, const int* counts, int n_counts,
+                                                                  long long rows, int mean, float* loss, int* count) {
+    __shared__ double sums[kSumThreads / 32];
+    __shared__ int ns[kSumThreads / 32];
+    const int tid = threadIdx.x;
+    double sum = 0;
+    int n = 0;
+    for (long long i = tid; i < rows; i += kSumThreads) {
+        sum += (double)losses[i];
+        if (stats) n += stats[i * kStats] != neg_inf();
+    }
+    if (counts && tid < n_counts) n = counts[tid];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+    n = __reduce_add_sync(~0u, n);
+    if ((tid & 31) == 0) {
+        sums[tid >> 5] = sum;
+        ns[tid >> 5] = n;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        sum = 0;
+        n = 0;
+        for (int w = 0; w < kSumThreads / 32; ++w) {
+            sum += sums[w];
+            n += ns[w];
+        }
+        loss[0] = (float)(mean ? sum / (n > 0 ? n : 1) : sum);
+        if (count) count[0] = n;
+    }
+}
+
+// ------------------------------------------------------------------ launches
+template <typename T, int MODE>
+static int distill_launch(DistillPlan p, int sm_count, cudaStream_t st) {
+    constexpr int ES = (int)sizeof(T), N = 16 / ES;
+    if (p.V + N - 1 <= kWarpElements) {
+        const size_t bytes = (size_t)kRowWarps * (32 + 3 * p.K) * 4;
+        distill_warp_kernel<T, MODE><<<(unsigned)((p.rows + kRowWarps - 1) / kRowWarps), 32 * kRowWarps, bytes, st>>>(p);
+    } else {
+        const long long row_bytes = (long long)p.V * ES;
+        long long slices = 1;
+        if (MODE == kGrad) {
+            // blocks on their own: 32 KB keep one for some microseconds, a sixteenth of that where there are few rows
+            slices = (row_bytes + 32767) / 32768;
+            while (p.rows * slices < 2 * sm_count && row_bytes / slices > 4096) slices *= 2;
+        } else {
+            // a cluster for each row: slices that fit shared memory, or, with few rows, more of them
+            while (slices < 8 && ((MODE == (kLoss | kGrad) && row_bytes / slices + 64 > kSliceBytes) ||
+                                  p.V / 8 / slices > kSliceBytes ||  // the bitmap
+                                  (p.rows * slices < 2 * sm_count && row_bytes / slices > 8192)))
+                slices *= 2;
+        }
+        long long per = (p.V + slices - 1) / slices;
+        per = (per + 7) / 8 * 8;  // granules of the slices keep the row's phase
+        slices = (p.V + per - 1) / per;
+        if (p.rows * slices > 0x7fffffffll) return DDF_B200_E_TOO_LARGE;
+        p.per = (int)per;
+        p.slices = (int)slices;
+        const size_t granules = (size_t)(per + N - 1) / N + 1;
+        const bool resident = MODE == (kLoss | kGrad) && granules * 16 <= kSliceBytes + 64;
+        const size_t bytes = (resident ? granules * 16 : 0) + (MODE & kLoss ? (granules * N + 31) / 32 * 4 : 0);
+        if (bytes > 200 * 1024) return DDF_B200_E_ARGUMENT;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(p.rows * slices));
+        cfg.blockDim = dim3(kRowThreads);
+        cfg.dynamicSmemBytes = bytes;
+        cfg.stream = st;
+        cudaLaunchAttribute attr = {};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = (unsigned)slices;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        if (MODE & kLoss) {
+            cfg.attrs = &attr;
+            cfg.numAttrs = slices > 1 ? 1 : 0;
+        }
+        auto kernel = resident ? distill_block_kernel<T, MODE, true> : distill_block_kernel<T, MODE, false>;
+        if (bytes > 40 * 1024) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+            if (e != cudaSuccess) return (int)e;
+        }
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+        if (e != cudaSuccess) return (int)e;
+    }
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return (int)cudaGetLastError();
+}
+
+template <int MODE> static int distill_dispatch(const DistillPlan& p, int dtype, int sm_count, cudaStream_t st) {
+    switch (dtype) {
+        case DDF_B200_F32: return distill_launch<float, MODE>(p, sm_count, st);
+        case DDF_B200_F16: return distill_launch<__half, MODE>(p, sm_count, st);
+        default: return distill_launch<__nv_bfloat16, MODE>(p, sm_count, st);
+    }
+}
+
+static int distill_check(const ddf_b200_distill_args* q, DistillPlan& p, int* sm) {
+    if (!q || !q->logits || !q->values || !q->indices) return DDF_B200_E_NULL;
+    if (q->rows < 1 || q->classes < 1 || q->k < 1 || q->row_stride < q->classes) return DDF_B200_E_ARGUMENT;
+    const float T = (float)q->temperature;
+    if (!(T > 0.f) || !(T <= 3.0e38f)) return DDF_B200_E_ARGUMENT;
+    if (q->k > kMaxTop) return DDF_B200_E_ARGUMENT;
+    if (q->classes > (1ll << 23) || q->rows > (1ll << 30)) return DDF_B200_E_TOO_LARGE;
+    for (int t : {q->dtype, q->values_dtype})
+        if (t != DDF_B200_F32 && t != DDF_B200_F16 && t != DDF_B200_BF16) return DDF_B200_E_DTYPE;
+    if (q->reduction < DDF_B200_NONE || q->reduction > DDF_B200_MEAN) return DDF_B200_E_ARGUMENT;
+    int index = 0, *fault = nullptr;
+    const int rc = device_facts(sm, &fault, &index);
+    if (rc) return rc;
+    p = DistillPlan{};
+    p.logits = q->logits; p.values = q->values; p.indices = q->indices; p.rest = q->rest;
+    p.stride = q->row_stride; p.rows = q->rows; p.V = (int)q->classes; p.K = q->k;
+    p.values_dtype = q->values_dtype; p.wide_indices = q->wide_indices;
+    p.c = (float)(1.4426950408889634 / q->temperature); p.T = T;
+    p.scale = 1.f; p.slices = 1;
+    return 0;
+}
+
+static int distill_sum(const float* losses, const float* stats, const int* counts, int n_counts, long long rows, int mean,
+                       float* loss, int* count, cudaStream_t st) {
+    distill_sum_kernel<<<1, kSumThreads, 0, st>>>(losses, stats, counts, n_counts, rows, mean, loss, count);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return (int)cudaGetLastError();
+}
+
+}  // namespace ddf
+
+extern "C" {
+
+int ddf_b200_distill_forward(const ddf_b200_distill_args* q, float* losses, float* stats, float* loss, int* count, void* stream) {
+    using namespace ddf;
+    DistillPlan p;
+    int sm = 0;
+    const int rc = distill_check(q, p, &sm);
+    if (rc) return rc;
+    if (!losses || !stats || (q->reduction != DDF_B200_NONE && (!loss || !count))) return DDF_B200_E_NULL;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    p.losses = losses;
+    p.stats = stats;
+    const int r = distill_dispatch<kLoss>(p, q->dtype, sm, st);
+    if (r || q->reduction == DDF_B200_NONE) return r;
+    return distill_sum(losses, stats, nullptr, 0, p.rows, q->reduction == DDF_B200_MEAN, loss, count, st);
+}
+
+int ddf_b200_distill_backward(const ddf_b200_distill_args* q, const float* stats, const int* count, const float* upstream,
+                              long long upstream_stride, void* grad, void* stream) {
+    using namespace ddf;
+    DistillPlan p;
+    int sm = 0;
+    const int rc = distill_check(q, p, &sm);
+    if (rc) return rc;
+    if (!stats || !upstream || !grad || (q->reduction == DDF_B200_MEAN && !count)) return DDF_B200_E_NULL;
+    p.stats = const_cast<float*>(stats);
+    p.upstream = upstream;
+    p.upstream_stride = upstream_stride;
+    p.counts = q->reduction == DDF_B200_MEAN ? count : nullptr;
+    p.n_counts = 1;
+    p.grad = grad;
+    return distill_dispatch<kGrad>(p, q->dtype, sm, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int ddf_b200_distill_loss_grad(const ddf_b200_distill_args* q, float* losses, int* counts, float* loss, double scale, void* grad,
+                               void* stream) {
+    using namespace ddf;
+    DistillPlan p;
+    int sm = 0;
+    const int rc = distill_check(q, p, &sm);
+    if (rc) return rc;
+    const bool mean = q->reduction == DDF_B200_MEAN;
+    if (!losses || !grad || (q->reduction != DDF_B200_NONE && !loss) || (mean && !counts)) return DDF_B200_E_NULL;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    p.losses = losses;
+    p.grad = grad;
+    p.scale = (float)scale;
+    if (mean) {
+        // the gradient needs the number of rows before any row's sum is known
+        p.n_counts = (int)(p.rows / 8 + 1 < kCountBlocks ? p.rows / 8 + 1 : kCountBlocks);
+        p.counts = counts;
+        distill_count_kernel<256><<<p.n_counts, 256, 0, st>>>(p, counts);
+        g_launches.fetch_add(1, std::memory_order_relaxed);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return (int)e;
+    }
+    const int r = distill_dispatch<kLoss | kGrad>(p, q->dtype, sm, st);
+    if (r || q->reduction == DDF_B200_NONE) return r;
+    return distill_sum(losses, nullptr, mean ? counts : nullptr, p.n_counts, p.rows, mean, loss, nullptr, st);
+}
+
+}  // extern "C"

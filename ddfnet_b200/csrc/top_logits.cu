@@ -1,0 +1,293 @@
+// A row's k largest logits, in order, and the log of what all its other classes sum to: the targets that a
+// teacher leaves for ddf_b200_distill (distill.cu).
+//
+//   values[n,i], indices[n,i]   the i-th largest of row n; equal ones by ascending class, NaN above all
+//   rest[n] = log sum over the classes j that are not among them of exp(x[n,j] / T)
+//
+// What bounds it: the row is read once from memory; everything after that works on its copy in shared memory
+// (rows up to kTopResident bytes) or reads it again out of L2.  One block per row.
+//   1. Every thread takes the largest of its share.  The k-th largest of these NT maxima bounds the row's
+//      k-th largest from below (k of the row's elements reach it), and is close: with m elements a thread
+//      about k + k^2 / (2 NT) elements lie at or above it.  A binary search over the upper 16 bits of the ordered
+//      keys finds it in 16 barriers that count.
+//   2. Elements at or above it go to a list; the others into the running softmax sum.
+//   3. Each listed element counts the elements ahead of it, by one 64-bit key (value, then lower class first):
+//      its place, or, past k, one more summand of the rest.
+// A list that runs over (rows of few distinct values, masked rows) takes the general way instead: a
+// radix selection of the k-th key over four histograms, then one ordered pass that fills in its equals.
+#include <atomic>
+
+#include "logits.cuh"
+
+namespace ddf {
+
+extern std::atomic<unsigned long long> g_launches;
+int device_facts(int* sm_count, int** fault, int* index);
+
+constexpr int kTopList = 1024;               // elements at or above the bound that are ranked directly
+constexpr int kTopResident = 72 * 1024;      // three blocks an SM keep their rows in shared memory
+
+// Order of the elements as an unsigned integer: -0 as +0, NaN on top.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x + 0.f);
+    if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+struct TopPlan {
+    const void* logits;
+    void* values;
+    long long* indices;
+    float* rest;
+    long long stride;
+    int V, k;
+    float c, T;
+};
+
+template <int NT> struct TopShared {
+    unsigned long long list[kTopList];
+    Online room[NT / 32];
+    int histogram[256];
+    int count, above, pick, warp_ties[NT / 32];
+};
+
+template <typename T, int NT, bool RESIDENT>
+__global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
+    constexpr int N = Granule<T>::N;
+    constexpr int UNROLL = 4;
+    extern __shared__ __align__(16) unsigned char copy_raw[];
+    uint4* copy = reinterpret_cast<uint4*>(copy_raw);
+    __shared__ TopShared<NT> sh;
+    const int tid = threadIdx.x;
+    const long long row = blockIdx.x;
+    const T* x = reinterpret_cast<const T*>(p.logits) + row * p.stride;
+    const Run<T> run(x, p.V);
+    const int last = run.granules - 1;
+    auto decode = [&](const uint4& raw, int g, float (&v)[N]) {
+        Granule<T>::get(raw, v);
+        if (g == 0 || g == last) {
+            const uint32_t out = run.outside(g);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (out >> i & 1u) v[i] = neg_inf();
+        }
+    };
+
+    if (tid == 0) sh.count = 0;
+    float most = neg_inf();
+    for (int g0 = tid; g0 < run.granules; g0 += NT * UNROLL) {
+        uint4 raw[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+            if (g0 + u * NT < run.granules) raw[u] = run.load(g0 + u * NT);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int g = g0 + u * NT;
+            if (g >= run.granules) break;
+            if constexpr (RESIDENT) copy[g] = raw[u];
+            float v[N];
+            decode(raw[u], g, v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) most = max_nan(most, v[i]);
+        }
+    }
+    uint32_t bound = 0;
+    const uint32_t mine = ordered(most) >> 16;
+#pragma unroll 1
+    for (uint32_t bit = 0x8000u; bit; bit >>= 1)
+        if (__syncthreads_count(mine >= (bound | bit)) >= p.k) bound |= bit;
+    const float floor_value = unordered(bound << 16);  // NaN where the search ends below -inf: every element passes
+
+    Online rest = Online::none();
+    for (int g = tid; g < run.granules; g += NT) {
+        float v[N];
+        decode(RESIDENT ? copy[g] : run.load(g), g, v);
+        float high = v[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) high = max_nan(high, v[i]);
+        if (!(high < floor_value)) {
+            const uint32_t out = run.outside(g);
+            high = neg_inf();
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (!(v[i] < floor_value)) {
+                    if (!(out >> i & 1u)) {
+                        const int at = atomicAdd(&sh.count, 1);
+                        if (at < kTopList)
+                            sh.list[at] = (unsigned long long)ordered(v[i]) << 32 | (0xffffffffu - (uint32_t)(g * N + i - run.phase));
+                    }
+                    v[i] = neg_inf();
+                }
+                high = max_nan(high, v[i]);
+            }
+        }
+        rest.add(v, high, p.c);
+    }
+    __syncthreads();
+    const int listed = sh.count;
+    T* values = reinterpret_cast<T*>(p.values) + row * p.k;
+    long long* indices = p.indices + row * p.k;
+    auto place = [&](int rank, uint32_t element) {
+        values[rank] = x[element];
+        indices[rank] = (long long)element;
+    };
+    if (listed <= kTopList) {
+        for (int i = tid; i < listed; i += NT) {
+            const unsigned long long key = sh.list[i];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < listed; ++j) rank += sh.list[j] > key;
+            if (rank < p.k) {
+                place(rank, 0xffffffffu - (uint32_t)key);
+            } else {
+                Online one;
+                one.m = unordered((uint32_t)(key >> 32));
+                if (one.m != neg_inf()) {
+                    if (isinf(one.m)) one.m = __int_as_float(0x7fc00000);  // a sum with +inf has no finite logarithm: as NaN
+                    one.ref = one.m;
+                    one.s = one.m == one.m ? 1.f : one.m;
+                    rest.merge(one, p.c);
+                }
+            }
+        }
+    } else {
+        // radix selection: the upper bytes of the k-th largest key, one histogram each
+        uint32_t prefix = 0;
+        int need = p.k;  // of the elements whose upper bytes equal the prefix
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            for (int i = tid; i < 256; i += NT) sh.histogram[i] = 0;
+            __syncthreads();
+            for (int g = tid; g < run.granules; g += NT) {
+                float v[N];
+                decode(RESIDENT ? copy[g] : run.load(g), g, v);
+                const uint32_t out = run.outside(g);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const uint32_t key = ordered(v[i]);
+                    if (!(out >> i & 1u) && (shift == 24 || (key ^ prefix) >> (shift + 8) == 0))
+                        atomicAdd(&sh.histogram[key >> shift & 255u], 1);
+                }
+            }
+            __syncthreads();
+            if (tid == 0) {
+                int above = 0, b = 255;
+                for (; b > 0 && above + sh.histogram[b] < need; --b) above += sh.histogram[b];
+                sh.pick = b;
+                sh.above = above;
+            }
+            __syncthreads();
+            prefix |= (uint32_t)sh.pick << shift;
+            need -= sh.above;
+            __syncthreads();
+        }
+        // `need` elements equal to the prefix belong to the list, those of the lowest classes
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+        rest = Online::none();
+        for (int g = tid; g < run.granules; g += NT) {
+            float v[N];
+            decode(RESIDENT ? copy[g] : run.load(g), g, v);
+            const uint32_t out = run.outside(g);
+            float high = neg_inf();
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const uint32_t key = ordered(v[i]);
+                if (key > prefix && !(out >> i & 1u))
+                    sh.list[atomicAdd(&sh.count, 1)] = (unsigned long long)key << 32 | (0xffffffffu - (uint32_t)(g * N + i - run.phase));
+                if (key >= prefix) v[i] = neg_inf();
+                high = max_nan(high, v[i]);
+            }
+            rest.add(v, high, p.c);
+        }
+        __syncthreads();
+        const int above = sh.count;  // k - need
+        for (int i = tid; i < above; i += NT) {
+            const unsigned long long key = sh.list[i];
+            int rank = 0;
+            for (int j = 0; j < above; ++j) rank += sh.list[j] > key;
+            place(rank, 0xffffffffu - (uint32_t)key);
+        }
+        // the equals in order of their classes; what is left of them belongs to the rest
+        int seen = 0, left = 0;
+        for (int e0 = 0; e0 < p.V; e0 += NT) {
+            const int e = e0 + tid;
+            const bool tie = e < p.V && ordered(Elem<T>::load(x + e)) == prefix;
+            const uint32_t votes = __ballot_sync(~0u, tie);
+            if ((tid & 31) == 0) sh.warp_ties[tid >> 5] = __popc(votes);
+            __syncthreads();
+            int before = seen + __popc(votes & ((1u << (tid & 31)) - 1u)), all = 0;
+#pragma unroll
+            for (int w = 0; w < NT / 32; ++w) {
+                if (w < tid >> 5) before += sh.warp_ties[w];
+                all += sh.warp_ties[w];
+            }
+            if (tie) {
+                if (before < need) place(above + before, (uint32_t)e);
+                else ++left;
+            }
+            seen += all;
+            __syncthreads();
+        }
+        const float tie = unordered(prefix);
+        if (left && tie != neg_inf()) {
+            Online some;
+            some.m = some.ref = tie;
+            some.s = isinf(tie) || !(tie == tie) ? __int_as_float(0x7fc00000) : (float)left;
+            rest.merge(some, p.c);
+        }
+    }
+    rest = block_merge<NT / 32>(rest, p.c, sh.room);
+    if (p.rest && tid == 0) p.rest[row] = rest.s == 0.f ? neg_inf() : rest.m / p.T + logf(rest.s);
+}
+
+template <typename T, int NT>
+static int top_launch(const TopPlan& p, long long rows, cudaStream_t st) {
+    const size_t bytes = ((size_t)p.V * sizeof(T) + 15) / 16 * 16 + 16;  // a granule more for a row that starts inside one
+    if (bytes <= kTopResident) {
+        if (bytes > 36 * 1024) {  // with the static part beyond what a block gets unasked
+            const cudaError_t e = cudaFuncSetAttribute(top_logits_kernel<T, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTopResident);
+            if (e != cudaSuccess) return (int)e;
+        }
+        top_logits_kernel<T, NT, true><<<(unsigned)rows, NT, bytes, st>>>(p);
+    } else {
+        top_logits_kernel<T, NT, false><<<(unsigned)rows, NT, 0, st>>>(p);
+    }
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return (int)cudaGetLastError();
+}
+
+template <typename T>
+static int top_choose(const TopPlan& p, long long rows, int sm_count, cudaStream_t st) {
+    const long long granules = (long long)p.V * (int)sizeof(T) / 16;
+    // k maxima must be there to bound the k-th largest
+    if (granules <= 512 && p.k <= 128) return top_launch<T, 128>(p, rows, st);
+    if (granules >= 4096 && rows <= sm_count) return top_launch<T, 1024>(p, rows, st);
+    return top_launch<T, 256>(p, rows, st);
+}
+
+}  // namespace ddf
+
+extern "C" int ddf_b200_top_logits(const void* logits, void* values, long long* indices, float* rest, long long rows,
+                                   long long classes, long long row_stride, int k, double temperature, int dtype,
+                                   void* stream) {
+    using namespace ddf;
+    if (!logits || !values || !indices) return DDF_B200_E_NULL;
+    if (rows < 1 || classes < 1 || k < 1 || k > classes || row_stride < classes) return DDF_B200_E_ARGUMENT;
+    if (!(temperature > 0) || !((float)temperature > 0.f) || !((float)temperature <= 3.0e38f)) return DDF_B200_E_ARGUMENT;
+    if (k > kMaxTop) return DDF_B200_E_ARGUMENT;
+    if (classes > (1ll << 30) || rows > 0x7fffffffll) return DDF_B200_E_TOO_LARGE;
+    int sm = 0, index = 0, *fault = nullptr;
+    const int rc = device_facts(&sm, &fault, &index);
+    if (rc) return rc;
+    TopPlan p{logits, values, indices, rest, row_stride, (int)classes, k, (float)(1.4426950408889634 / temperature), (float)temperature};
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case DDF_B200_F32: return top_choose<float>(p, rows, sm, st);
+        case DDF_B200_F16: return top_choose<__half>(p, rows, sm, st);
+        case DDF_B200_BF16: return top_choose<__nv_bfloat16>(p, rows, sm, st);
+        default: return DDF_B200_E_DTYPE;
+    }
+}

@@ -1,0 +1,198 @@
+"""Distillation of a classifier from a teacher's top logits.
+
+``top_logits``         the targets: a teacher's k largest logits of each row, their classes, and the log of what
+                       all other classes sum to.
+``distill_loss``       the loss of a student's logits against them, with its gradient through autograd.
+``distill_loss_grad``  loss and gradient in one call that reads the logits once, for training loops that know the
+                       loss's upstream gradient (a loss scale, a chunk of a large head).
+
+The mathematics stands in include/ddf_b200.h and csrc/distill.cu.  Logits are float32, float16 or bfloat16 CUDA
+tensors of any leading shape whose last dimension is the classes; sums and losses are float32.  Rows may lie any
+number of elements apart; other layouts are copied first.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_REDUCTIONS = {"none": _lib.NONE, "sum": _lib.SUM, "mean": _lib.MEAN}
+_MOST_ENTRIES = 256
+
+
+class TopLogits(NamedTuple):
+    values: torch.Tensor   # (..., k), the logits' type, descending
+    indices: torch.Tensor  # (..., k), int64
+    rest: torch.Tensor     # (...), float32: log of the other classes' sum of exp(logit / temperature)
+
+
+def _rows(logits):
+    """`logits` as (rows, classes) with unit stride along the classes and rows that do not overlap."""
+    classes = logits.shape[-1]
+    flat = logits.reshape(-1, classes)
+    if flat.shape[0] and ((classes > 1 and flat.stride(1) != 1) or (flat.shape[0] > 1 and flat.stride(0) < classes)):
+        flat = flat.contiguous()
+    return flat
+
+
+def _check_logits(logits, what):
+    if not logits.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor")
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"{what}: float32, float16 or bfloat16, not {logits.dtype}")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{what} of shape {tuple(logits.shape)} has no classes")
+
+
+def _check_temperature(temperature):
+    temperature = float(temperature)
+    if not 0.0 < temperature <= 3e38:
+        raise ValueError(f"temperature must be positive and finite, not {temperature}")
+    return temperature
+
+
+def _row_stride(flat):
+    return flat.stride(0) if flat.shape[0] > 1 else flat.shape[1]
+
+
+def top_logits(logits, k, temperature=1.0):
+    """The k (at most 256) largest ``logits`` of each row in descending order, equal ones by ascending class and
+    NaN above all numbers; and the log of the others' sum of ``exp(logit / temperature)``.  Records no gradient."""
+    _check_logits(logits, "logits")
+    temperature = _check_temperature(temperature)
+    classes, k = logits.shape[-1], int(k)
+    if not 1 <= k <= min(classes, _MOST_ENTRIES):
+        raise ValueError(f"k must be from 1 to {min(classes, _MOST_ENTRIES)}, not {k}")
+    lead, dev = logits.shape[:-1], logits.device
+    flat = _rows(logits.detach())
+    values = torch.empty(*lead, k, dtype=logits.dtype, device=dev)
+    indices = torch.empty(*lead, k, dtype=torch.int64, device=dev)
+    rest = torch.empty(lead, dtype=torch.float32, device=dev)
+    if flat.shape[0]:
+        with torch.cuda.device(dev):
+            _lib.check(_lib.load().ddf_b200_top_logits(
+                flat.data_ptr(), values.data_ptr(), indices.data_ptr(), rest.data_ptr(), flat.shape[0], classes,
+                _row_stride(flat), k, temperature, _DTYPES[logits.dtype], torch.cuda.current_stream().cuda_stream))
+    return TopLogits(values, indices, rest)
+
+
+def _check_targets(logits, values, indices, rest, reduction):
+    _check_logits(logits, "logits")
+    lead = logits.shape[:-1]
+    if values.dtype not in _DTYPES:
+        raise TypeError(f"values: float32, float16 or bfloat16, not {values.dtype}")
+    if indices.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"indices: int32 or int64, not {indices.dtype}")
+    if values.shape != indices.shape or values.dim() < 1 or values.shape[:-1] != lead:
+        raise ValueError(f"values {tuple(values.shape)} and indices {tuple(indices.shape)} do not match "
+                         f"logits {tuple(logits.shape)}")
+    if not 1 <= values.shape[-1] <= _MOST_ENTRIES:
+        raise ValueError(f"from 1 to {_MOST_ENTRIES} entries a row, not {values.shape[-1]}")
+    if rest is not None and (rest.shape != lead or not rest.is_floating_point()):
+        raise ValueError(f"rest must be floating point of shape {tuple(lead)}, not {rest.dtype} {tuple(rest.shape)}")
+    for t in (values, indices, rest):
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"the targets must be on {logits.device}, not {t.device}")
+        if t is not None and t.requires_grad:
+            raise ValueError("the teacher's values take no gradient: detach them")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be 'none', 'sum' or 'mean', not {reduction!r}")
+
+
+def _args(flat, values, indices, rest, temperature, reduction):
+    return _lib.DistillArgs(
+        flat.data_ptr(), values.data_ptr(), indices.data_ptr(), rest.data_ptr() if rest is not None else None,
+        flat.shape[0], flat.shape[1], _row_stride(flat), values.shape[-1], _DTYPES[flat.dtype], _DTYPES[values.dtype],
+        int(indices.dtype == torch.int64), _REDUCTIONS[reduction], temperature)
+
+
+class DistillFunction(Function):
+    @staticmethod
+    def forward(ctx, logits, values, indices, rest, temperature, reduction):
+        lead, dev = logits.shape[:-1], logits.device
+        flat = _rows(logits)
+        values, indices = values.contiguous(), indices.contiguous()
+        rest = rest.to(torch.float32).contiguous() if rest is not None else None
+        n = flat.shape[0]
+        losses = torch.empty(lead, dtype=torch.float32, device=dev)
+        if n == 0:
+            ctx.empty = True
+            ctx.shape, ctx.dtype = logits.shape, logits.dtype
+            return losses if reduction == "none" else torch.zeros((), dtype=torch.float32, device=dev)
+        ctx.empty = False
+        stats = torch.empty(n, _lib.DISTILL_STATS, dtype=torch.float32, device=dev)
+        loss = count = None
+        if reduction != "none":
+            loss = torch.empty((), dtype=torch.float32, device=dev)
+            count = torch.empty(1, dtype=torch.int32, device=dev)
+        args = _args(flat, values, indices, rest, temperature, reduction)
+        with torch.cuda.device(dev):
+            _lib.check(_lib.load().ddf_b200_distill_forward(
+                ctypes.byref(args), losses.data_ptr(), stats.data_ptr(), loss.data_ptr() if loss is not None else None,
+                count.data_ptr() if count is not None else None, torch.cuda.current_stream().cuda_stream))
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(flat, values, indices, rest, stats, count)
+            ctx.shape, ctx.temperature, ctx.reduction = logits.shape, temperature, reduction
+        return losses if reduction == "none" else loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, upstream):
+        if ctx.empty:
+            return torch.zeros(ctx.shape, dtype=ctx.dtype, device=upstream.device), None, None, None, None, None
+        flat, values, indices, rest, stats, count = ctx.saved_tensors
+        grad = torch.empty(ctx.shape, dtype=flat.dtype, device=flat.device)
+        upstream = upstream.to(torch.float32)
+        if ctx.reduction == "none" and not upstream.is_contiguous():
+            upstream = upstream.contiguous()
+        args = _args(flat, values, indices, rest, ctx.temperature, ctx.reduction)
+        with torch.cuda.device(flat.device):
+            _lib.check(_lib.load().ddf_b200_distill_backward(
+                ctypes.byref(args), stats.data_ptr(), count.data_ptr() if count is not None else None,
+                upstream.data_ptr(), int(ctx.reduction == "none"), grad.data_ptr(),
+                torch.cuda.current_stream().cuda_stream))
+        return grad, None, None, None, None, None
+
+
+def distill_loss(logits, values, indices, rest=None, temperature=1.0, reduction="mean"):
+    """T^2 times the Kullback-Leibler divergence of the student's softmax from the teacher's, at temperature T, over
+    the classes that the teacher lists (``values``, ``indices`` of shape (..., k)) and, with ``rest``, all others
+    together: ``distill_loss(student, *top_logits(teacher, k, T), temperature=T)``.
+
+    Without ``rest`` the teacher's softmax is over its listed classes alone.  An index outside the classes is an
+    empty entry; a row of nothing else does not count (loss and gradient 0, left out of the mean).  Returns a
+    float32 scalar, or, with ``reduction='none'``, one loss a row; the gradient goes to ``logits`` alone."""
+    _check_targets(logits, values, indices, rest, reduction)
+    return DistillFunction.apply(logits, values, indices, rest, _check_temperature(temperature), reduction)
+
+
+def distill_loss_grad(logits, values, indices, rest=None, temperature=1.0, reduction="mean", scale=1.0):
+    """``(loss, gradient)``: what ``distill_loss`` returns, and ``scale`` times its gradient with respect to
+    ``logits`` (with ``reduction='none'``: that of the losses' sum), contiguous and of their type.  Reads the logits
+    once.  Records no autograd history."""
+    _check_targets(logits, values, indices, rest, reduction)
+    temperature = _check_temperature(temperature)
+    lead, dev = logits.shape[:-1], logits.device
+    flat = _rows(logits.detach())
+    losses = torch.empty(lead, dtype=torch.float32, device=dev)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    n = flat.shape[0]
+    if n == 0:
+        return (losses if reduction == "none" else torch.zeros((), dtype=torch.float32, device=dev)), grad
+    values, indices = values.contiguous(), indices.contiguous()
+    rest = rest.to(torch.float32).contiguous() if rest is not None else None
+    loss = torch.empty((), dtype=torch.float32, device=dev) if reduction != "none" else None
+    counts = torch.empty(_lib.DISTILL_COUNTS, dtype=torch.int32, device=dev) if reduction == "mean" else None
+    args = _args(flat, values, indices, rest, temperature, reduction)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().ddf_b200_distill_loss_grad(
+            ctypes.byref(args), losses.data_ptr(), counts.data_ptr() if counts is not None else None,
+            loss.data_ptr() if loss is not None else None, float(scale), grad.data_ptr(),
+            torch.cuda.current_stream().cuda_stream))
+    return (losses if reduction == "none" else loss), grad

@@ -64,6 +64,7 @@ extern "C" {
 #define DDF_B200_E_DEVICE (-10)     /* no usable CUDA device / not an sm_100 device    */
 #define DDF_B200_E_SCRATCH_LIMIT (-11) /* ddf_b200_backward_noalloc: problem needs more
                                           scratch than the built-in array holds          */
+#define DDF_B200_E_ARGUMENT (-12)   /* an argument is outside the range its declaration states */
 
 /* Library version: major*10000 + minor*100 + patch. */
 int ddf_b200_version(void);
@@ -350,6 +351,71 @@ int ddf_b200_channel_filter(const float* pooled, int n_partials, float pool_scal
  * a pixel's C values, x and y must be 16-byte aligned (DDF_B200_E_UNSUPPORTED otherwise).
  */
 int ddf_b200_maxpool_nhwc(const void* x, void* y, int B, int C, int H, int W, int dtype, void* stream);
+
+/*
+ * Distillation of a classifier from a teacher's top logits (no counterpart in the reference, whose
+ * training script knows hard labels only).
+ *
+ * ddf_b200_top_logits: of each row of logits (rows x classes, `row_stride` elements apart) the k largest
+ * as values (rows x k, of the logits' type) and indices (rows x k), in descending order, equal ones by
+ * ascending class, NaN above all numbers; and, where rest is not NULL,
+ *   rest[n] = log sum over the other classes of exp(logit / temperature),
+ * -inf where there is none (NaN where NaN or +inf is among them).  k <= 256.  dtype F32, F16 or BF16.
+ */
+int ddf_b200_top_logits(const void* logits, void* values, long long* indices, float* rest, long long rows,
+                        long long classes, long long row_stride, int k, double temperature, int dtype,
+                        void* stream);
+
+/* how the rows' losses are put together */
+#define DDF_B200_NONE 0 /* they are not: one loss a row              */
+#define DDF_B200_SUM 1
+#define DDF_B200_MEAN 2 /* over the rows that count (see below)      */
+
+/*
+ * The loss.  Row n's classes fall into k + 1 buckets, the listed ones and all others together; with
+ * a_i = values[n,i] / T and a_rest = rest[n] (rest NULL: -inf), b_i = logits[n, indices[n,i]] / T and
+ * b_rest = log sum over the others of exp(logits[n,j] / T), p = softmax(a) and q = softmax(b),
+ *   loss_n = T^2 sum p log(p / q),
+ *   d loss_n / d logits[n,j] = T (q_i - p_i) for a listed class,
+ *                              T (q_rest - p_rest) exp(logits[n,j] / T - b_rest) for the others.
+ * Without rest that is the cross entropy of the teacher's softmax over its top classes, less its entropy.
+ * An index outside [0, classes) is an empty entry; a class listed twice has the sum of its
+ * probabilities.  A row with no entry, or whose teacher values are all -inf, does not count: its loss
+ * is 0, its gradients are 0.  The mean over no row is 0.
+ * values (rows x k) may be of another type than the logits; indices are int, or long long with
+ * wide_indices; both contiguous.  k <= 256, classes <= 2^23.
+ */
+typedef struct ddf_b200_distill_args {
+    const void* logits;
+    const void* values;
+    const void* indices;
+    const float* rest; /* or NULL */
+    long long rows, classes, row_stride;
+    int k;
+    int dtype, values_dtype; /* F32, F16 or BF16 */
+    int wide_indices;
+    int reduction;
+    double temperature; /* > 0 */
+} ddf_b200_distill_args;
+
+/* floats of `stats` a row */
+#define DDF_B200_DISTILL_STATS 8
+/* ints of `counts` */
+#define DDF_B200_DISTILL_COUNTS 128
+
+/* Forward: losses (rows floats), stats (rows x DDF_B200_DISTILL_STATS floats, 16-byte aligned, for the
+ * backward) and, for SUM and MEAN, loss[0] and the number of rows that count in count[0]. */
+int ddf_b200_distill_forward(const ddf_b200_distill_args* args, float* losses, float* stats, float* loss,
+                             int* count, void* stream);
+/* Backward: grad (rows x classes, contiguous, of the logits' type) from the forward's stats and count.
+ * Row n's upstream gradient is upstream[n * upstream_stride] (stride 0: one for all). */
+int ddf_b200_distill_backward(const ddf_b200_distill_args* args, const float* stats, const int* count,
+                              const float* upstream, long long upstream_stride, void* grad, void* stream);
+/* Both in one pass over the logits, for a training loop that knows its upstream gradient (`scale`):
+ * losses, loss[0] (SUM, MEAN) and grad = scale * d loss / d logits; for NONE every row's loss has the
+ * upstream gradient `scale`.  counts: DDF_B200_DISTILL_COUNTS ints of scratch (MEAN). */
+int ddf_b200_distill_loss_grad(const ddf_b200_distill_args* args, float* losses, int* counts, float* loss,
+                               double scale, void* grad, void* stream);
 
 /*
  * Reads and clears the per-device fault word that the streaming kernels set
