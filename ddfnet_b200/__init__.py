@@ -12,7 +12,9 @@ from ._lib import take_fault
 from .host import ddf_host, ddf_host_async
 from .layout import to_channels_last, to_nchw
 from .distill import TopLogits, distill_loss, distill_loss_grad, top_logits
+from .linear import linear_act
 
 __all__ = ["ddf", "ddf_sfnorm", "DDFFunction", "DDFSpatialNormFunction", "DDFPack", "DDFUpPack", "FilterNorm",
            "build_spatial_branch", "build_channel_branch", "ddf_host", "ddf_host_async", "to_nchw",
-           "to_channels_last", "take_fault", "top_logits", "TopLogits", "distill_loss", "distill_loss_grad"]
+           "to_channels_last", "take_fault", "top_logits", "TopLogits", "distill_loss", "distill_loss_grad",
+           "linear_act"]

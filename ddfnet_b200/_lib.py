@@ -31,6 +31,15 @@ class DistillArgs(ctypes.Structure):
                 ("temperature", ctypes.c_double)]
 
 
+class LinearArgs(ctypes.Structure):
+    """ddf_b200_linear_args"""
+    _fields_ = [("x", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+                ("residual", ctypes.c_void_p), ("rows", ctypes.c_longlong), ("inputs", ctypes.c_longlong),
+                ("outputs", ctypes.c_longlong), ("x_stride", ctypes.c_longlong), ("weight_stride", ctypes.c_longlong),
+                ("residual_stride", ctypes.c_longlong), ("activation", ctypes.c_int), ("after", ctypes.c_int),
+                ("dtype", ctypes.c_int)]
+
+
 # every symbol include/ddf_b200.h declares
 SYMBOLS = (
     "ddf_b200_version", "ddf_b200_strerror", "ddf_b200_forward", "ddf_b200_plan",
@@ -42,6 +51,8 @@ SYMBOLS = (
     "ddf_b200_forward_nhwc", "ddf_b200_nhwc_waitlimit", "ddf_b200_pool_nhwc_tiles", "ddf_b200_pool_nhwc",
     "ddf_b200_sfnorm", "ddf_b200_sfnorm_backward", "ddf_b200_maxpool_nhwc",
     "ddf_b200_top_logits", "ddf_b200_distill_forward", "ddf_b200_distill_backward", "ddf_b200_distill_loss_grad",
+    "ddf_b200_linear_workspace", "ddf_b200_linear_forward", "ddf_b200_linear_backward_workspace",
+    "ddf_b200_linear_backward",
     "ddf_b200_noop", "ddf_b200_rate_probe_bytes", "ddf_b200_rate_probe",
 )
 
@@ -93,6 +104,15 @@ def load() -> ctypes.CDLL:
         L.ddf_b200_distill_backward.argtypes = [args, vp, vp, vp, ll, vp, vp]
         L.ddf_b200_distill_loss_grad.restype = i
         L.ddf_b200_distill_loss_grad.argtypes = [args, vp, vp, vp, ctypes.c_double, vp, vp]
+        linear = ctypes.POINTER(LinearArgs)
+        L.ddf_b200_linear_workspace.restype = sz
+        L.ddf_b200_linear_workspace.argtypes = [linear]
+        L.ddf_b200_linear_forward.restype = i
+        L.ddf_b200_linear_forward.argtypes = [linear, vp, vp, vp, sz, vp]
+        L.ddf_b200_linear_backward_workspace.restype = sz
+        L.ddf_b200_linear_backward_workspace.argtypes = [linear, vp, ll] + [vp] * 4
+        L.ddf_b200_linear_backward.restype = i
+        L.ddf_b200_linear_backward.argtypes = [linear, vp, ll] + [vp] * 6 + [sz, vp]
         L.ddf_b200_sfnorm.restype = i
         L.ddf_b200_sfnorm.argtypes = [vp, vp] + [i] * 5 + [ctypes.c_double, vp]
         L.ddf_b200_sfnorm_backward.restype = i

@@ -1,0 +1,454 @@
+// linear_act: checks, choice of kernels and launches, and the kernels around the products: few rows, operands
+// that TMA cannot address, the activation's gradient with the bias's column sums.
+#include <atomic>
+
+#include "linear.cuh"
+
+namespace ddf {
+
+extern std::atomic<unsigned long long> g_launches;
+int device_facts(int* sm_count, int** fault, int* index);
+
+static int launched() {
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return (int)cudaGetLastError();
+}
+
+// ------------------------------------------------------------------ few rows
+// y (M <= MR rows): a warp, or four of them with a quarter of K each, per CW columns; W is read once, 16 bytes a
+// lane, x out of L1.  Bound by W's bytes; with more rows than this the tensor cores' tiles are faster although
+// most of their rows are empty.
+constexpr int kRowsWarps = 4;
+
+template <typename T, int MR, int CW, bool SPLIT, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kRowsWarps) linear_rows_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w, long long ldw, int M, int N, int K, const Epilogue e) {
+    constexpr int V = ALIGNED ? 8 : 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int col0 = (SPLIT ? blockIdx.x : blockIdx.x * kRowsWarps + warp) * CW;
+    __shared__ float sums[kRowsWarps][MR * CW];
+    if (col0 >= N) return;  // (a block's warps leave together where they split K)
+    float acc[MR][CW] = {};
+    const T* wp[CW];
+#pragma unroll
+    for (int c = 0; c < CW; ++c) wp[c] = w + (long long)min(col0 + c, N - 1) * ldw;
+    constexpr int STEP = 32 * V * (SPLIT ? kRowsWarps : 1);
+    const int first = (SPLIT ? warp * 32 + lane : lane) * V;
+#pragma unroll 2
+    for (int k = first; k < K; k += STEP) {
+        float a[CW][V];
+        if constexpr (ALIGNED) {
+#pragma unroll
+            for (int c = 0; c < CW; ++c) {
+                uint4 g;
+                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(g.x), "=r"(g.y), "=r"(g.z), "=r"(g.w) : "l"(wp[c] + k));
+                const uint32_t q[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[c][i] = Word<T>::get(q[i / 2], i % 2);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < CW; ++c) a[c][0] = Elem<T>::load(wp[c] + k);
+        }
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+            const T* xp = x + (long long)min(m, M - 1) * ldx + k;
+            float b[V];
+            if constexpr (ALIGNED) {
+                const uint4 g = __ldg(reinterpret_cast<const uint4*>(xp));
+                const uint32_t q[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) b[i] = Word<T>::get(q[i / 2], i % 2);
+            } else {
+                b[0] = Elem<T>::load(xp);
+            }
+#pragma unroll
+            for (int c = 0; c < CW; ++c)
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[m][c] = fmaf(a[c][i], b[i], acc[m][c]);
+        }
+    }
+    float mine = 0.f;  // lane l finishes element l
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int c = 0; c < CW; ++c) {
+            float v = acc[m][c];
+#pragma unroll
+            for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+            if (lane == m * CW + c) mine = v;
+        }
+    if constexpr (SPLIT) {
+        if (lane < MR * CW) sums[warp][lane] = mine;
+        __syncthreads();
+        if (warp) return;
+        if (lane < MR * CW) {
+            mine = 0.f;
+#pragma unroll
+            for (int s = 0; s < kRowsWarps; ++s) mine += sums[s][lane];
+        }
+    }
+    const int m = lane / CW, col = col0 + lane % CW;
+    if (lane >= MR * CW || m >= M || col >= N) return;
+    float z[4] = {mine, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f};
+    if (e.bias) b[0] = Elem<T>::load(reinterpret_cast<const T*>(e.bias) + col);
+    if (e.residual) r[0] = Elem<T>::load(reinterpret_cast<const T*>(e.residual) + (long long)m * e.ldr + col);
+    finish4<T>(e, m, col, 1, z, b, r);
+}
+
+// ------------------------------------------------------------------ operands that TMA cannot address
+// Rows that do not start on 16 bytes: copied to rows that do.
+template <typename T> __global__ void __launch_bounds__(256) linear_pack_kernel(const T* __restrict__ src, long long ld, T* __restrict__ dst, long long ldp, long long rows, int cols) {
+    for (long long row = blockIdx.y * 8 + (threadIdx.x >> 5); row < rows; row += (long long)gridDim.y * 8)
+#pragma unroll 4
+        for (int c = blockIdx.x * 128 + (threadIdx.x & 31), i = 0; i < 4; ++i, c += 32)
+            if (c < cols) dst[row * ldp + c] = __ldg(src + row * ld + c);
+}
+
+// ------------------------------------------------------------------ backward of what follows the product
+// gz = gy act'(.) into up to two buffers, and its sums over `chunk` rows of each column.  Bound by bytes: gy and
+// aux read once, gz written once.  A warp takes 128 columns of a row at a time.
+struct BackPlan {
+    const void *gy, *aux;
+    void *gz, *gz2;    // either may be NULL; rows ldz / N apart
+    float* sums;       // chunks x N, or NULL
+    long long ldg, ldz, M;
+    int N, act, chunk, vec, vecz;
+};
+template <typename T> __global__ void __launch_bounds__(256) linear_back_kernel(const BackPlan p) {
+    __shared__ float4 sums[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int col = blockIdx.x * 128 + lane * 4, left = p.N - col;
+    const long long r0 = (long long)blockIdx.y * p.chunk, r1 = min(p.M, r0 + p.chunk);
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (left > 0) {
+#pragma unroll 4
+        for (long long r = r0 + warp; r < r1; r += 8) {
+            float g[4], z[4];
+            load4(reinterpret_cast<const T*>(p.gy) + r * p.ldg + col, p.vec, left, g);
+            if (p.act != kActNone) {
+                load4(reinterpret_cast<const T*>(p.aux) + r * p.N + col, p.vec, left, z);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) g[i] *= act_slope(z[i], p.act);
+            }
+            if (p.gz) store4(reinterpret_cast<T*>(p.gz) + r * p.ldz + col, p.vecz, left, g);
+            if (p.gz2) store4(reinterpret_cast<T*>(p.gz2) + r * p.N + col, p.vec, left, g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += g[i];
+        }
+    }
+    if (!p.sums) return;
+    sums[warp][lane] = make_float4(s[0], s[1], s[2], s[3]);
+    __syncthreads();
+    if (threadIdx.x < 128) {
+        const int c = blockIdx.x * 128 + threadIdx.x;
+        float all = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) all += reinterpret_cast<const float*>(&sums[w][0])[threadIdx.x];
+        if (c < p.N) p.sums[(long long)blockIdx.y * p.N + c] = all;
+    }
+}
+// Column sums of the chunks' sums, in one order.
+template <typename T> __global__ void __launch_bounds__(256) linear_bias_kernel(const float* __restrict__ sums, T* __restrict__ gb, int chunks, int N) {
+    __shared__ float part[8][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    float s = 0.f;
+    if (c < N)
+#pragma unroll 4
+        for (int i = warp; i < chunks; i += 8) s += __ldg(sums + (long long)i * N + c);
+    part[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < N) {
+        s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += part[w][lane];
+        Elem<T>::store(gb + c, s);
+    }
+}
+
+// ------------------------------------------------------------------ host side
+// cuTensorMapEncodeTiled, from the driver that the runtime has loaded (the library links no driver).
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled() {
+    static std::atomic<EncodeTiled> known{nullptr};
+    EncodeTiled f = known.load(std::memory_order_acquire);
+    if (!f) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) return nullptr;
+        f = reinterpret_cast<EncodeTiled>(p);
+        known.store(f, std::memory_order_release);
+    }
+    return f;
+}
+
+// A matrix whose rows TMA can address: `rows` of `cols` elements, `ld` apart.
+struct Matrix {
+    const void* p;
+    long long rows, cols, ld;
+};
+static bool addressable(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
+static long long padded(long long n) { return (n + 7) / 8 * 8; }
+
+static int encode(CUtensorMap* map, const Matrix& m, int dtype, int box_rows) {
+    const EncodeTiled f = encode_tiled();
+    if (!f) return DDF_B200_E_DEVICE;
+    const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.ld * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, unit[2] = {1, 1};
+    return f(map, dtype == DDF_B200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(m.p), dims, strides, box,
+             unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : DDF_B200_E_ARGUMENT;
+}
+
+// How a product is cut: columns of a tile and splits of K.
+struct Cut {
+    int bn, splits, steps;
+};
+static Cut cut_of(long long M, long long N, long long K, int sm_count) {
+    const long long steps = (K + kTileK - 1) / kTileK, tiles_m = (M + kTileM - 1) / kTileM;
+    Cut best{256, 1, (int)steps};
+    double least = 1e300;
+    for (int bn : {256, 128, 64}) {
+        if (bn > 64 && N <= bn / 2) continue;
+        // clocks of a step of 64 along K, and of a tile's start and end
+        const double step = bn == 256 ? 600 : bn == 128 ? 370 : 260, once = 1200 + 5 * bn;
+        const long long tiles = tiles_m * ((N + bn - 1) / bn);
+        for (int want = 1; want <= 32; ++want) {
+            const long long per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
+            if (splits != want) continue;
+            if (splits > 1 && (per < 4 || (double)splits * M * N > 64e6)) break;
+            const long long waves = (tiles * splits + sm_count - 1) / sm_count;
+            const double join = splits > 1 ? 4000 + (double)M * N * (8 * splits + 4) / 3000 : 0;
+            const double cost = (double)waves * (per * step + once) + join;
+            if (cost < least * 0.97) {
+                least = cost;
+                best = Cut{bn, (int)splits, (int)per};
+            }
+        }
+    }
+    return best;
+}
+static size_t partial_bytes(long long M, long long N, const Cut& c) { return c.splits > 1 ? (size_t)c.splits * M * N * 4 : 0; }
+
+// D (M x N) = A B^T.  at / bt: the matrix given is stored with the reduction as its rows.
+template <typename T, bool AT, bool BT>
+static int product(const Matrix& a, const Matrix& b, long long M, long long N, long long K, const Epilogue& out, float* partial, int dtype, long long limit,
+                   cudaStream_t st) {
+    int sm = 0, index = 0, *fault = nullptr;
+    int rc = device_facts(&sm, &fault, &index);
+    if (rc) return rc;
+    const Cut cut = cut_of(M, N, K, sm);
+    auto kernel = cut.bn == 256 ? linear_kernel<T, 256, AT, BT> : cut.bn == 128 ? linear_kernel<T, 128, AT, BT> : linear_kernel<T, 64, AT, BT>;
+    // (before the driver's encoder: a runtime call gives a thread that has none its context)
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinearShared);
+    if (e != cudaSuccess) return (int)e;
+    LinearPlan p{};
+    if ((rc = encode(&p.a, a, dtype, AT ? kTileK : kTileM))) return rc;
+    if ((rc = encode(&p.b, b, dtype, BT ? kTileK : cut.bn))) return rc;
+    p.out = out;
+    p.partial = cut.splits > 1 ? partial : nullptr;
+    p.M = (int)M; p.N = (int)N; p.K = (int)K;
+    p.tiles_m = (int)((M + kTileM - 1) / kTileM);
+    p.tiles_n = (int)((N + cut.bn - 1) / cut.bn);
+    p.splits = cut.splits;
+    p.steps = cut.steps;
+    const uint32_t type = dtype == DDF_B200_BF16 ? 1u : 0u;
+    p.idesc = 1u << 4 | type << 7 | type << 10 | (AT ? 1u << 15 : 0u) | (BT ? 1u << 16 : 0u) | (uint32_t)(cut.bn / 8) << 17 | (uint32_t)(kTileM / 16) << 24;
+    p.fault = fault;
+    p.limit = limit;
+    const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
+    if (items > 0x7fffffffll) return DDF_B200_E_TOO_LARGE;
+    kernel<<<(unsigned)(items < sm ? items : sm), kLinearThreads, kLinearShared, st>>>(p);
+    rc = launched();
+    if (rc || cut.splits == 1) return rc;
+    linear_join_kernel<T><<<(unsigned)((M * ((N + 3) / 4) + 255) / 256), 256, 0, st>>>(partial, out, (int)M, (int)N, cut.splits);
+    return launched();
+}
+
+constexpr int kFewRows = 4;
+
+template <typename T, int MR, int CW> static int rows_launch(const ddf_b200_linear_args* q, const Epilogue& e, cudaStream_t st) {
+    const bool aligned = q->inputs % 8 == 0 && addressable(q->x, q->rows > 1 ? q->x_stride : 0) && addressable(q->weight, q->outputs > 1 ? q->weight_stride : 0);
+    const long long cols = (q->outputs + CW - 1) / CW;
+    const bool split = q->inputs >= 1024 && cols < 148 * 16;  // too few warps to keep the memory busy
+    auto kernel = split ? (aligned ? linear_rows_kernel<T, MR, CW, true, true> : linear_rows_kernel<T, MR, CW, true, false>)
+                        : (aligned ? linear_rows_kernel<T, MR, CW, false, true> : linear_rows_kernel<T, MR, CW, false, false>);
+    kernel<<<(unsigned)(split ? cols : (cols + kRowsWarps - 1) / kRowsWarps), 32 * kRowsWarps, 0, st>>>(
+        (const T*)q->x, q->x_stride, (const T*)q->weight, q->weight_stride, (int)q->rows, (int)q->outputs, (int)q->inputs, e);
+    return launched();
+}
+
+template <typename T> static int pack(const Matrix& m, void* to, cudaStream_t st) {
+    const long long tall = (m.rows + 7) / 8;
+    linear_pack_kernel<T><<<dim3((unsigned)((m.cols + 127) / 128), (unsigned)(tall < 32768 ? tall : 32768)), 256, 0, st>>>((const T*)m.p, m.ld, (T*)to, padded(m.cols), m.rows, (int)m.cols);
+    return launched();
+}
+
+// Workspace: consecutive blocks, 256-byte aligned.
+struct Space {
+    char* base;
+    size_t used = 0;
+    void* take(size_t bytes) {
+        void* p = base ? base + used : nullptr;
+        used += (bytes + 255) / 256 * 256;
+        return p;
+    }
+};
+
+static int check_linear(const ddf_b200_linear_args* q) {
+    if (!q || !q->x || !q->weight) return DDF_B200_E_NULL;
+    if (q->rows < 1 || q->inputs < 1 || q->outputs < 1 || q->x_stride < q->inputs || q->weight_stride < q->inputs) return DDF_B200_E_ARGUMENT;
+    if (q->rows > (1ll << 30) || q->inputs > (1ll << 24) || q->outputs > (1ll << 24)) return DDF_B200_E_TOO_LARGE;
+    if (q->activation < DDF_B200_ACT_NONE || q->activation > DDF_B200_ACT_SILU) return DDF_B200_E_ARGUMENT;
+    if (q->residual && q->residual_stride < q->outputs) return DDF_B200_E_ARGUMENT;
+    if (q->dtype != DDF_B200_F16 && q->dtype != DDF_B200_BF16) return DDF_B200_E_DTYPE;
+    return 0;
+}
+static bool by_four(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0 && ld % 4 == 0; }
+
+template <typename T>
+static int forward(const ddf_b200_linear_args* q, void* y, void* aux, Space& ws, size_t have, long long limit, cudaStream_t st, bool only_size, int sm) {
+    const long long M = q->rows, N = q->outputs, K = q->inputs;
+    Epilogue e{y, aux, q->bias, q->residual, N, q->residual_stride, q->activation, q->after, 0};
+    e.vec = by_four(y, N) && (!aux || by_four(aux, N)) && (!q->residual || by_four(q->residual, q->residual_stride));
+    if (M <= kFewRows && limit == kWaitCycles) {
+        if (only_size) return 0;
+        if (M == 1) return rows_launch<T, 1, 1>(q, e, st);
+        if (M == 2) return rows_launch<T, 2, 1>(q, e, st);
+        return rows_launch<T, 4, 2>(q, e, st);
+    }
+    Matrix x{q->x, M, K, q->x_stride}, w{q->weight, N, K, q->weight_stride};
+    void* xp = addressable(x.p, x.ld) ? nullptr : ws.take((size_t)M * padded(K) * 2);
+    const bool pack_x = !addressable(x.p, x.ld), pack_w = !addressable(w.p, w.ld);
+    void* wp = pack_w ? ws.take((size_t)N * padded(K) * 2) : nullptr;
+    float* partial = (float*)ws.take(partial_bytes(M, N, cut_of(M, N, K, sm)));
+    if (only_size) return 0;
+    if (ws.used > have) return DDF_B200_E_WORKSPACE;
+    int rc;
+    if (pack_x) {
+        if ((rc = pack<T>(x, xp, st))) return rc;
+        x.p = xp; x.ld = padded(K);
+    }
+    if (pack_w) {
+        if ((rc = pack<T>(w, wp, st))) return rc;
+        w.p = wp; w.ld = padded(K);
+    }
+    return product<T, false, false>(x, w, M, N, K, e, partial, q->dtype, limit, st);
+}
+
+template <typename T>
+static int backward(const ddf_b200_linear_args* q, const void* gy, long long gy_stride, const void* aux, void* gx, void* gw, void* gb, void* gr, Space& ws,
+                    size_t have, cudaStream_t st, bool only_size, int sm) {
+    const long long M = q->rows, N = q->outputs, K = q->inputs;
+    const bool products = gx || gw;
+    const bool act = q->activation != DDF_B200_ACT_NONE;
+    // gz in rows that TMA can address: gy itself, the residual's gradient (gz, where it precedes the activation), or the workspace
+    const bool want_gr = gr && !q->after;
+    const bool as_gy = !act && addressable(gy, gy_stride), as_gr = !as_gy && want_gr && addressable(gr, N);
+    const bool scratch = products && !as_gy && !as_gr;
+    Matrix gz{as_gy ? gy : as_gr ? gr : nullptr, M, N, as_gy ? gy_stride : as_gr ? N : padded(N)};
+    void* gzp = scratch ? ws.take((size_t)M * padded(N) * 2) : nullptr;
+    if (scratch) gz.p = gzp;
+    const long long most = 256;  // chunks of rows for the column sums
+    long long chunk = (M + most - 1) / most;
+    chunk = chunk < 64 ? 64 : (chunk + 7) / 8 * 8;
+    const long long chunks = (M + chunk - 1) / chunk;
+    float* sums = gb ? (float*)ws.take((size_t)chunks * N * 4) : nullptr;
+    Matrix x{q->x, M, K, q->x_stride}, w{q->weight, N, K, q->weight_stride};
+    const bool pack_x = gw && !addressable(x.p, x.ld), pack_w = gx && !addressable(w.p, w.ld);
+    void* xp = pack_x ? ws.take((size_t)M * padded(K) * 2) : nullptr;
+    void* wp = pack_w ? ws.take((size_t)N * padded(K) * 2) : nullptr;
+    size_t need = 0;
+    if (gx) need = partial_bytes(M, K, cut_of(M, K, N, sm));
+    if (gw) {
+        const size_t n = partial_bytes(N, K, cut_of(N, K, M, sm));
+        need = n > need ? n : need;
+    }
+    float* partial = (float*)ws.take(need);
+    if (only_size) return 0;
+    if (ws.used > have) return DDF_B200_E_WORKSPACE;
+
+    int rc;
+    if (scratch || want_gr || gb) {
+        BackPlan b{gy, aux, scratch ? gzp : nullptr, want_gr ? gr : nullptr, sums, gy_stride, padded(N), M, (int)N, q->activation, (int)chunk, 0, 0};
+        b.vec = by_four(gy, gy_stride) && (!act || by_four(aux, N)) && (!want_gr || by_four(gr, N));
+        b.vecz = 1;
+        linear_back_kernel<T><<<dim3((unsigned)((N + 127) / 128), (unsigned)chunks), 256, 0, st>>>(b);
+        if ((rc = launched())) return rc;
+        if (gb) {
+            linear_bias_kernel<T><<<(unsigned)((N + 31) / 32), 256, 0, st>>>(sums, (T*)gb, (int)chunks, (int)N);
+            if ((rc = launched())) return rc;
+        }
+    }
+    if (pack_x) {
+        if ((rc = pack<T>(x, xp, st))) return rc;
+        x.p = xp; x.ld = padded(K);
+    }
+    if (pack_w) {
+        if ((rc = pack<T>(w, wp, st))) return rc;
+        w.p = wp; w.ld = padded(K);
+    }
+    Epilogue e{};
+    if (gx) {
+        e.y = gx; e.ldy = K; e.vec = by_four(gx, K);
+        if ((rc = product<T, false, true>(gz, w, M, K, N, e, partial, q->dtype, kWaitCycles, st))) return rc;
+    }
+    if (gw) {
+        e.y = gw; e.ldy = K; e.vec = by_four(gw, K);
+        if ((rc = product<T, true, true>(gz, x, N, K, M, e, partial, q->dtype, kWaitCycles, st))) return rc;
+    }
+    return 0;
+}
+
+}  // namespace ddf
+
+extern "C" {
+
+size_t ddf_b200_linear_workspace(const ddf_b200_linear_args* q) {
+    using namespace ddf;
+    int sm = 0, index = 0, *fault = nullptr;
+    if (check_linear(q) || device_facts(&sm, &fault, &index)) return 0;
+    Space ws{nullptr};
+    forward<__half>(q, nullptr, nullptr, ws, 0, kWaitCycles, nullptr, true, sm);
+    return ws.used;
+}
+
+int ddf_b200_linear_forward(const ddf_b200_linear_args* q, void* y, void* aux, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace ddf;
+    int rc = check_linear(q);
+    if (rc) return rc;
+    if (!y || (workspace_bytes && !workspace)) return DDF_B200_E_NULL;
+    int sm = 0, index = 0, *fault = nullptr;
+    if ((rc = device_facts(&sm, &fault, &index))) return rc;
+    Space ws{(char*)workspace};
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return q->dtype == DDF_B200_F16 ? forward<__half>(q, y, aux, ws, workspace_bytes, kWaitCycles, st, false, sm)
+                                    : forward<__nv_bfloat16>(q, y, aux, ws, workspace_bytes, kWaitCycles, st, false, sm);
+}
+
+size_t ddf_b200_linear_backward_workspace(const ddf_b200_linear_args* q, const void* gy, long long gy_stride, const void* gx, const void* gw, const void* gb,
+                                          const void* gr) {
+    using namespace ddf;
+    int sm = 0, index = 0, *fault = nullptr;
+    if (check_linear(q) || device_facts(&sm, &fault, &index)) return 0;
+    Space ws{nullptr};
+    backward<__half>(q, gy, gy_stride, nullptr, const_cast<void*>(gx), const_cast<void*>(gw), const_cast<void*>(gb), const_cast<void*>(gr), ws, 0, nullptr, true, sm);
+    return ws.used;
+}
+
+int ddf_b200_linear_backward(const ddf_b200_linear_args* q, const void* gy, long long gy_stride, const void* aux, void* gx, void* gw, void* gb, void* gr,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace ddf;
+    int rc = check_linear(q);
+    if (rc) return rc;
+    if (!gy || (q->activation != DDF_B200_ACT_NONE && !aux) || (workspace_bytes && !workspace)) return DDF_B200_E_NULL;
+    if (gy_stride < q->outputs) return DDF_B200_E_ARGUMENT;
+    int sm = 0, index = 0, *fault = nullptr;
+    if ((rc = device_facts(&sm, &fault, &index))) return rc;
+    Space ws{(char*)workspace};
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return q->dtype == DDF_B200_F16 ? backward<__half>(q, gy, gy_stride, aux, gx, gw, gb, gr, ws, workspace_bytes, st, false, sm)
+                                    : backward<__nv_bfloat16>(q, gy, gy_stride, aux, gx, gw, gb, gr, ws, workspace_bytes, st, false, sm);
+}
+
+}  // extern "C"

@@ -1,0 +1,128 @@
+"""``linear_act``: a matrix product with bias, residual and activation in its epilogue, forward and backward, on the
+tensor cores (csrc/linear.cuh).  What a classifier and the 1x1 convolutions of a channels_last network are:
+``x.permute(0, 2, 3, 1)`` of a channels_last tensor has a row for each pixel.
+
+float16 and bfloat16 CUDA tensors, all of one type; sums are float, results are rounded once.  Under autocast the
+arguments are cast to its type.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .distill import _row_stride, _rows
+
+_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def _args(x, weight, bias, residual, activation, after):
+    ptr = lambda t: t.data_ptr() if t is not None else None
+    return _lib.LinearArgs(
+        x.data_ptr(), weight.data_ptr(), ptr(bias), ptr(residual), x.shape[0], x.shape[1], weight.shape[0],
+        _row_stride(x), _row_stride(weight), _row_stride(residual) if residual is not None else 0,
+        _ACTIVATIONS[activation], int(after), _DTYPES[x.dtype])
+
+
+def _scratch(size, device):
+    return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+
+
+class LinearActFunction(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation, after):
+        lead, n, dev = x.shape[:-1], weight.shape[0], x.device
+        flat, weight = _rows(x), _rows(weight)
+        bias = bias.contiguous() if bias is not None else None
+        res = _rows(residual) if residual is not None else None
+        y = torch.empty(*lead, n, dtype=x.dtype, device=dev)
+        grad = any(ctx.needs_input_grad)
+        # what the activation's slope is taken at: its input, or, where a ReLU ends the call, its output
+        aux = None
+        if grad and activation != "none" and (activation != "relu" or (after and residual is not None)):
+            aux = torch.empty_like(y)
+        if y.numel():
+            lib, args = _lib.load(), _args(flat, weight, bias, res, activation, after)
+            with torch.cuda.device(dev):
+                ws, size = _scratch(lib.ddf_b200_linear_workspace(ctypes.byref(args)), dev)
+                _lib.check(lib.ddf_b200_linear_forward(
+                    ctypes.byref(args), y.data_ptr(), aux.data_ptr() if aux is not None else None,
+                    ws.data_ptr() if ws is not None else None, size, torch.cuda.current_stream().cuda_stream))
+        if grad:
+            if activation == "relu" and aux is None:
+                aux = y
+            ctx.save_for_backward(flat, weight, aux)
+            ctx.shape, ctx.activation, ctx.after, ctx.has_residual = x.shape, activation, after, residual is not None
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, weight, aux = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        n, k, dev = weight.shape[0], x.shape[1], x.device
+        flat = _rows(gy.to(x.dtype))
+        gx = torch.empty(ctx.shape, dtype=x.dtype, device=dev) if need_x else None
+        gw = torch.empty(n, k, dtype=x.dtype, device=dev) if need_w else None
+        gb = torch.empty(n, dtype=x.dtype, device=dev) if need_b else None
+        # a residual behind the activation, or of a call without one, has the gradient that arrives
+        through = ctx.after or ctx.activation == "none"
+        gr = torch.empty(gy.shape, dtype=x.dtype, device=dev) if need_r and not through else None
+        if flat.numel() and (need_x or need_w or need_b or gr is not None):
+            lib, args = _lib.load(), _args(x, weight, None, None, ctx.activation, ctx.after)
+            ptr = lambda t: t.data_ptr() if t is not None else None
+            outs = [ptr(t) for t in (gx, gw, gb, gr)]
+            with torch.cuda.device(dev):
+                ws, size = _scratch(lib.ddf_b200_linear_backward_workspace(
+                    ctypes.byref(args), flat.data_ptr(), _row_stride(flat), *outs), dev)
+                _lib.check(lib.ddf_b200_linear_backward(
+                    ctypes.byref(args), flat.data_ptr(), _row_stride(flat), ptr(aux), *outs, ptr(ws), size,
+                    torch.cuda.current_stream().cuda_stream))
+        elif not flat.numel():
+            for t in (gx, gw, gb, gr):
+                if t is not None:
+                    t.zero_()
+        if need_r and through:
+            gr = gy
+        return gx, gw, gb, gr, None, None
+
+
+def _check(x, weight, bias, residual, activation, add):
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"linear_act: float16 or bfloat16, not {x.dtype}")
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
+        raise ValueError(f"weight {tuple(weight.shape)} does not match x {tuple(x.shape)}")
+    n = weight.shape[0]
+    if bias is not None and bias.shape != (n,):
+        raise ValueError(f"bias {tuple(bias.shape)} does not match weight {tuple(weight.shape)}")
+    if residual is not None and residual.shape != (*x.shape[:-1], n):
+        raise ValueError(f"residual {tuple(residual.shape)} does not match the output {(*x.shape[:-1], n)}")
+    for t in (weight, bias, residual):
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError(f"linear_act: all of one type, not {x.dtype} and {t.dtype}")
+        if t is not None and t.device != x.device:
+            raise ValueError(f"all arguments must be on {x.device}, not {t.device}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, not {activation!r}")
+    if add not in ("before", "after"):
+        raise ValueError(f"add must be 'before' or 'after', not {add!r}")
+
+
+def linear_act(x, weight, bias=None, residual=None, activation="none", add="before"):
+    """``act(x @ weight.T + bias + residual)``, or, with ``add='after'``, ``act(x @ weight.T + bias) + residual``.
+
+    ``x`` (..., inputs), ``weight`` (outputs, inputs), ``bias`` (outputs), ``residual`` (..., outputs);
+    ``activation`` 'none', 'relu', 'gelu' (by erf) or 'silu'.  Rows may lie any number of elements apart.  Gradients go
+    to every tensor; the activation's input is kept for them in the tensors' type."""
+    if torch.is_autocast_enabled("cuda") and x.is_cuda:
+        dt = torch.get_autocast_dtype("cuda")
+        x, weight, bias, residual = (t.to(dt) if t is not None and t.is_floating_point() else t
+                                     for t in (x, weight, bias, residual))
+    _check(x, weight, bias, residual, activation, add)
+    return LinearActFunction.apply(x, weight, bias, residual, activation, add == "after")

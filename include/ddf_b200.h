@@ -418,6 +418,48 @@ int ddf_b200_distill_loss_grad(const ddf_b200_distill_args* args, float* losses,
                                double scale, void* grad, void* stream);
 
 /*
+ * Matrix product with bias, residual and activation in its epilogue (the reference leaves its
+ * classifier, ddf_resnet.py, and the 1x1 convolutions to library calls):
+ *   z = x W^T + bias [+ residual];  y = act(z) [+ residual]
+ * x (rows x inputs), weight (outputs x inputs), bias (outputs) or NULL, residual (rows x outputs) or
+ * NULL, added before the activation or, with `after`, behind it; y (rows x outputs, contiguous).  All of
+ * one 2-byte type (F16, BF16); strides in elements between rows, at least the row's length; sums in
+ * float, one rounding on the store.  A channels_last tensor is such an x: a row for each pixel.
+ * rows <= 2^30, inputs and outputs <= 2^24.
+ *
+ * aux (rows x outputs, contiguous, or NULL): receives z for the backward, rounded to the type as a stored
+ * activation input is.  Where the activation is RELU and no residual follows it, y serves as well.
+ */
+#define DDF_B200_ACT_NONE 0
+#define DDF_B200_ACT_RELU 1
+#define DDF_B200_ACT_GELU 2 /* z Phi(z), by erf */
+#define DDF_B200_ACT_SILU 3 /* z / (1 + exp(-z)) */
+typedef struct ddf_b200_linear_args {
+    const void *x, *weight, *bias, *residual;
+    long long rows, inputs, outputs;
+    long long x_stride, weight_stride, residual_stride;
+    int activation, after, dtype;
+} ddf_b200_linear_args;
+
+/* Bytes of scratch, 256-byte aligned: rows that do not start on 16 bytes are copied there, and splits of
+ * the inputs axis leave partial sums.  0 is possible. */
+size_t ddf_b200_linear_workspace(const ddf_b200_linear_args* args);
+int ddf_b200_linear_forward(const ddf_b200_linear_args* args, void* y, void* aux, void* workspace,
+                            size_t workspace_bytes, void* stream);
+/*
+ * Backward, from the gradient gy (rows gy_stride apart) and aux (ACT_NONE: not read):
+ *   gz = gy act'(z);  gx = gz W;  gw = gz^T x;  gb = column sums of gz;  gr = gz
+ * each contiguous, of the type, or NULL.  (gr of a residual that follows the activation is gy itself and
+ * is not written.)  gz is rounded to the type: it is the products' operand.  bias and residual of args
+ * are not read.
+ */
+size_t ddf_b200_linear_backward_workspace(const ddf_b200_linear_args* args, const void* gy, long long gy_stride,
+                                          const void* gx, const void* gw, const void* gb, const void* gr);
+int ddf_b200_linear_backward(const ddf_b200_linear_args* args, const void* gy, long long gy_stride,
+                             const void* aux, void* gx, void* gw, void* gb, void* gr, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
  * Reads and clears the per-device fault word that the streaming kernels set
  * when one of their bounded waits runs out (they then stop instead of spinning).
  * Synchronises the device.  0 = no fault recorded; otherwise a positive code
