@@ -1,8 +1,8 @@
 """Builds libddf_b200.so from the CUDA sources in this directory with nvcc for
 sm_100a (cross-compiles without a GPU).  The library links the CUDA runtime
 statically and has no other dependency, so it loads in any process.
-Then builds _native.so (native.cpp, g++ against the installed torch): the host
-path of the Python operator.
+Then builds _native.so (native.cpp, native_head.cpp; g++ against the installed torch):
+the host path of the Python operators.
 
     python -m ddfnet_b200.csrc.build [--force] [-DNAME=VALUE ...] [--out NAME]
 """
@@ -84,20 +84,25 @@ def build(force: bool = False, defines: list[str] | None = None,
     return out
 
 
+NATIVE_SOURCES = ["native.cpp", "native_head.cpp"]
+
+
 def build_native(force: bool = False) -> str:
-    """Compiles native.cpp into ddfnet_b200/_native.so."""
+    """Compiles the C++ host path (NATIVE_SOURCES) into ddfnet_b200/_native.so."""
     import sysconfig
 
     import torch
-    src, out = os.path.join(HERE, "native.cpp"), os.path.join(PKG, "_native.so")
+    out = os.path.join(PKG, "_native.so")
     root = os.path.dirname(os.path.abspath(torch.__file__))
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{cuda}/include",
-           f"-I{sysconfig.get_paths()['include']}", src, "-o", out + ".tmp", f"-L{root}/lib",
-           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{root}/lib"]
-    h = hashlib.sha256((" ".join(cmd) + torch.__version__).encode())
-    for p in (src, os.path.join(os.path.dirname(PKG), "include", "ddf_b200.h")):
+    compile_cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-c",
+                   f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{cuda}/include",
+                   f"-I{sysconfig.get_paths()['include']}"]
+    link_cmd = ["g++", "-shared", "-o", out + ".tmp", f"-L{root}/lib", "-Wl,--no-as-needed",
+                "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{root}/lib"]
+    h = hashlib.sha256((" ".join(compile_cmd + link_cmd) + torch.__version__).encode())
+    for p in [os.path.join(HERE, f) for f in NATIVE_SOURCES + ["native.h"]] + [
+            os.path.join(os.path.dirname(PKG), "include", "ddf_b200.h")]:
         with open(p, "rb") as f:
             h.update(f.read())
     stamp = out + ".stamp"
@@ -105,9 +110,21 @@ def build_native(force: bool = False) -> str:
         with open(stamp) as f:
             if f.read() == h.hexdigest():
                 return out
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    bdir = os.path.join(HERE, "build", "native")
+    os.makedirs(bdir, exist_ok=True)
+
+    def compile_one(src: str) -> str:
+        obj = os.path.join(bdir, src.replace(".cpp", ".o"))
+        r = subprocess.run(compile_cmd + [os.path.join(HERE, src), "-o", obj], capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed on {src}:\n{r.stderr}")
+        return obj
+
+    with cf.ThreadPoolExecutor(max_workers=len(NATIVE_SOURCES)) as ex:
+        objs = list(ex.map(compile_one, NATIVE_SOURCES))
+    r = subprocess.run(link_cmd + objs, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed on native.cpp:\n{r.stderr}")
+        raise RuntimeError(f"linking _native.so failed:\n{r.stderr}")
     os.replace(out + ".tmp", out)
     with open(stamp, "w") as f:
         f.write(h.hexdigest())

@@ -12,42 +12,14 @@
 // batch's output in the graph as a constant), functorch transforms, dispatch modes and forward mode.
 //
 // The library's entry points are bound by address (bind()), so DDF_B200_LIB keeps working.
-#include <Python.h>
+#include "native.h"
 
-#include <ATen/ATen.h>
-#include <ATen/SequenceNumber.h>
-#include <ATen/cuda/CUDAGraphsUtils.cuh>
-#include <ATen/cuda/EmptyTensor.h>
-#include <ATen/record_function.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/saved_variable.h>
+namespace ddf_native {
 
-#include <cstring>
-#include <string>
-
-#include "../../include/ddf_b200.h"
+Library lib;
 
 namespace {
 
-using at::Tensor;
-
-// ------------------------------------------------------------------ bound entry points
-struct Library {
-    decltype(&ddf_b200_forward) forward = nullptr;
-    decltype(&ddf_b200_forward_sfnorm) forward_sfnorm = nullptr;
-    decltype(&ddf_b200_backward_workspace) backward_workspace = nullptr;
-    decltype(&ddf_b200_backward) backward = nullptr;
-    decltype(&ddf_b200_sfnorm) sfnorm = nullptr;
-    decltype(&ddf_b200_sfnorm_backward) sfnorm_backward = nullptr;
-    decltype(&ddf_b200_maxpool_nhwc) maxpool_nhwc = nullptr;
-    decltype(&ddf_b200_take_fault) take_fault = nullptr;
-} lib;
 PyObject* g_error_class = nullptr;  // _lib.DDFError
 PyObject* g_general = nullptr;      // op._general
 PyObject* g_load = nullptr;         // op._bind_native: loads the library and calls bind()
@@ -59,8 +31,8 @@ bool g_debug = false;
     throw e;
 }
 
-// A non-zero status becomes _lib.DDFError(status); with DDF_B200_DEBUG=1 the fault word is read
-// after every call.  Called without the GIL.
+}  // namespace
+
 void check(int status) {
     if (C10_LIKELY(status == 0 && !g_debug)) return;
     if (status != 0) {
@@ -77,21 +49,7 @@ void check(int status) {
                                  "); the output of the last call is incomplete");
 }
 
-int dtype_code(at::ScalarType t) {
-    switch (t) {
-        case at::kFloat: return DDF_B200_F32;
-        case at::kHalf: return DDF_B200_F16;
-        case at::kBFloat16: return DDF_B200_BF16;
-        case at::kDouble: return DDF_B200_F64;
-        default: return -1;
-    }
-}
-
-Tensor empty_like_on(at::IntArrayRef sizes, at::ScalarType dt, const at::Device& dev) {
-    return at::detail::empty_cuda(sizes, dt, dev, std::nullopt);
-}
-
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+namespace {
 
 // ------------------------------------------------------------------ one call's parameters
 struct Params {
@@ -184,8 +142,6 @@ bool plain_int(PyObject* o, int& v) {
     return true;
 }
 
-bool text_is(PyObject* o, const char* s) { return PyUnicode_Check(o) && PyUnicode_CompareWithASCIIString(o, s) == 0; }
-
 // The reference's argument checks (ddf/ddf.py:32-65); false: `general` finds out which one failed.
 bool parse(PyObject* const* args, Py_ssize_t n, bool norm, Params& p, const Tensor*& x, const Tensor*& cf,
            const Tensor*& sf, at::ScalarType& dt) {
@@ -230,7 +186,8 @@ bool parse(PyObject* const* args, Py_ssize_t n, bool norm, Params& p, const Tens
     return dtype_code(dt) >= 0;
 }
 
-// Nothing watches or transforms the program (see the head of this file).
+}  // namespace
+
 bool ordinary(std::initializer_list<const Tensor*> tensors) {
     using c10::DispatchKey;
     // set while a thread traces, has a dispatch mode, is inside a functorch transform
@@ -242,13 +199,14 @@ bool ordinary(std::initializer_list<const Tensor*> tensors) {
     return true;
 }
 
-// Loads and binds the library on the first call; false: a Python error is set.
 bool loaded() {
     if (C10_LIKELY(lib.forward != nullptr)) return true;
     PyObject* r = PyObject_CallNoArgs(g_load);
     Py_XDECREF(r);
     return r != nullptr;
 }
+
+namespace {
 
 PyObject* call(PyObject* const* args, Py_ssize_t n, bool norm) {
     HANDLE_TH_ERRORS
@@ -372,7 +330,12 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     if (!get("ddf_b200_forward", l.forward) || !get("ddf_b200_forward_sfnorm", l.forward_sfnorm) ||
         !get("ddf_b200_backward_workspace", l.backward_workspace) || !get("ddf_b200_backward", l.backward) ||
         !get("ddf_b200_sfnorm", l.sfnorm) || !get("ddf_b200_sfnorm_backward", l.sfnorm_backward) ||
-        !get("ddf_b200_take_fault", l.take_fault) || !get("ddf_b200_maxpool_nhwc", l.maxpool_nhwc)) {
+        !get("ddf_b200_take_fault", l.take_fault) || !get("ddf_b200_maxpool_nhwc", l.maxpool_nhwc) ||
+        !get("ddf_b200_top_logits", l.top_logits) || !get("ddf_b200_distill_forward", l.distill_forward) ||
+        !get("ddf_b200_distill_backward", l.distill_backward) || !get("ddf_b200_distill_loss_grad", l.distill_loss_grad) ||
+        !get("ddf_b200_linear_workspace", l.linear_workspace) || !get("ddf_b200_linear_forward", l.linear_forward) ||
+        !get("ddf_b200_linear_backward_workspace", l.linear_backward_workspace) ||
+        !get("ddf_b200_linear_backward", l.linear_backward)) {
         PyErr_SetString(PyExc_KeyError, "bind: an entry point is missing");
         return nullptr;
     }
@@ -396,5 +359,13 @@ PyMethodDef methods[] = {
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
+}  // namespace ddf_native
 
-PyMODINIT_FUNC PyInit__native(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__native(void) {
+    PyObject* m = PyModule_Create(&ddf_native::module);
+    if (m && !ddf_native::add_head(m)) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

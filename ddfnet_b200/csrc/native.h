@@ -1,0 +1,80 @@
+// What the translation units of the C++ host path (native.cpp, native_head.cpp) share: the library's entry points,
+// bound by address, errors, and the test for an ordinary call.
+#pragma once
+
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <ATen/SequenceNumber.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <ATen/cuda/EmptyTensor.h>
+#include <ATen/record_function.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
+
+#include <cstring>
+#include <string>
+
+#include "../../include/ddf_b200.h"
+
+namespace ddf_native {
+
+using at::Tensor;
+
+// ------------------------------------------------------------------ bound entry points
+struct Library {
+    decltype(&ddf_b200_forward) forward = nullptr;
+    decltype(&ddf_b200_forward_sfnorm) forward_sfnorm = nullptr;
+    decltype(&ddf_b200_backward_workspace) backward_workspace = nullptr;
+    decltype(&ddf_b200_backward) backward = nullptr;
+    decltype(&ddf_b200_sfnorm) sfnorm = nullptr;
+    decltype(&ddf_b200_sfnorm_backward) sfnorm_backward = nullptr;
+    decltype(&ddf_b200_maxpool_nhwc) maxpool_nhwc = nullptr;
+    decltype(&ddf_b200_take_fault) take_fault = nullptr;
+    decltype(&ddf_b200_top_logits) top_logits = nullptr;
+    decltype(&ddf_b200_distill_forward) distill_forward = nullptr;
+    decltype(&ddf_b200_distill_backward) distill_backward = nullptr;
+    decltype(&ddf_b200_distill_loss_grad) distill_loss_grad = nullptr;
+    decltype(&ddf_b200_linear_workspace) linear_workspace = nullptr;
+    decltype(&ddf_b200_linear_forward) linear_forward = nullptr;
+    decltype(&ddf_b200_linear_backward_workspace) linear_backward_workspace = nullptr;
+    decltype(&ddf_b200_linear_backward) linear_backward = nullptr;
+};
+extern Library lib;
+
+// A non-zero status becomes _lib.DDFError(status); with DDF_B200_DEBUG=1 the fault word is read
+// after every call.  Called without the GIL.
+void check(int status);
+// Loads and binds the library on the first call; false: a Python error is set.
+bool loaded();
+// Nothing watches or transforms the program (see the head of native.cpp).
+bool ordinary(std::initializer_list<const Tensor*> tensors);
+
+inline int dtype_code(at::ScalarType t) {
+    switch (t) {
+        case at::kFloat: return DDF_B200_F32;
+        case at::kHalf: return DDF_B200_F16;
+        case at::kBFloat16: return DDF_B200_BF16;
+        case at::kDouble: return DDF_B200_F64;
+        default: return -1;
+    }
+}
+
+inline Tensor empty_like_on(at::IntArrayRef sizes, at::ScalarType dt, const at::Device& dev) {
+    return at::detail::empty_cuda(sizes, dt, dev, std::nullopt);
+}
+
+inline void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+inline bool text_is(PyObject* o, const char* s) { return PyUnicode_Check(o) && PyUnicode_CompareWithASCIIString(o, s) == 0; }
+
+// Adds the functions of native_head.cpp to the module.
+bool add_head(PyObject* module);
+
+}  // namespace ddf_native

@@ -1,0 +1,411 @@
+// The host path in C++ of top_logits, distill_loss, distill_loss_grad and linear_act: as native.cpp, for the ordinary
+// call -- arguments that pass the checks below, plain tensors in rows that the library takes as they are, nothing that
+// watches or transforms the program.  For every other call the functions return None, and the caller (distill.py,
+// linear.py) takes its autograd function, which raises the errors, copies what needs copying and follows autocast.
+#include "native.h"
+
+#include <ATen/autocast_mode.h>
+
+namespace ddf_native {
+namespace {
+
+// `t` as rows of its last dimension a fixed number of elements apart.
+struct Rows {
+    int64_t rows = 1, cols = 0, stride = 0;
+    bool of(const Tensor& t) {
+        const int64_t d = t.dim();
+        if (d < 1 || t.numel() == 0) return false;
+        cols = t.size(d - 1);
+        if (cols > 1 && t.stride(d - 1) != 1) return false;
+        rows = t.numel() / cols;
+        stride = cols;
+        int64_t expect = -1;  // of the next dimension outwards
+        for (int64_t i = d - 2; i >= 0; --i) {
+            if (t.size(i) == 1) continue;
+            if (expect < 0) stride = t.stride(i);
+            else if (t.stride(i) != expect) return false;
+            expect = t.stride(i) * t.size(i);
+        }
+        return stride >= cols;
+    }
+};
+
+bool leading_is(const Tensor& t, const Tensor& of, int64_t extra) {  // t.shape == of.shape[:-1] + extra dimensions
+    const auto a = t.sizes(), b = of.sizes();
+    if (a.size() != b.size() - 1 + extra) return false;
+    for (size_t i = 0; i + 1 < b.size(); ++i)
+        if (a[i] != b[i]) return false;
+    return true;
+}
+
+const Tensor* tensor_or_none(PyObject* o, bool& ok) {  // nullptr for None
+    if (o == Py_None) return nullptr;
+    if (!THPVariable_Check(o)) { ok = false; return nullptr; }
+    return &THPVariable_Unpack(o);
+}
+
+bool number(PyObject* o, double& v) {
+    v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+    return true;
+}
+
+bool logits_dtype(const Tensor& t) {
+    const auto s = t.scalar_type();
+    return s == at::kFloat || s == at::kHalf || s == at::kBFloat16;
+}
+
+bool usual_temperature(double t) { return t > 1e-30 && t < 1e30; }
+
+void* stream_of(const at::Device& dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+
+std::vector<int64_t> leading(const Tensor& t) { return std::vector<int64_t>(t.sizes().begin(), t.sizes().end() - 1); }
+
+// ------------------------------------------------------------------ top_logits(logits, k, temperature)
+PyObject* py_top_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    double temperature;
+    if (n != 3 || !THPVariable_Check(args[0]) || !PyLong_CheckExact(args[1]) || !number(args[2], temperature)) Py_RETURN_NONE;
+    const Tensor& x = THPVariable_Unpack(args[0]);
+    const long k = PyLong_AsLong(args[1]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    Rows r;
+    if (!x.is_cuda() || !logits_dtype(x) || !ordinary({&x}) || !r.of(x) || k < 1 || k > 256 || k > r.cols || !usual_temperature(temperature))
+        Py_RETURN_NONE;
+    if (!loaded()) return nullptr;
+    Tensor values, indices, rest;
+    {
+        pybind11::gil_scoped_release no_gil;
+        RECORD_FUNCTION("top_logits", std::vector<c10::IValue>({x}));
+        const at::Device dev = x.device();
+        c10::cuda::CUDAGuard on_device(dev);
+        auto sizes = leading(x);
+        rest = empty_like_on(sizes, at::kFloat, dev);
+        sizes.push_back(k);
+        values = empty_like_on(sizes, x.scalar_type(), dev);
+        indices = empty_like_on(sizes, at::kLong, dev);
+        check(lib.top_logits(x.data_ptr(), values.data_ptr(), static_cast<long long*>(indices.data_ptr()), rest.data_ptr<float>(), r.rows, r.cols, r.stride, (int)k,
+                             temperature, dtype_code(x.scalar_type()), stream_of(dev)));
+    }
+    PyObject* out = PyTuple_New(3);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(values)));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(indices)));
+    PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::move(rest)));
+    return out;
+    END_HANDLE_TH_ERRORS
+}
+
+// ------------------------------------------------------------------ the distillation loss
+// (logits, values, indices, rest or None, temperature, reduction)
+struct Distill {
+    const Tensor *x, *values, *indices, *rest;
+    ddf_b200_distill_args args;
+
+    bool parse(PyObject* const* a) {
+        bool ok = THPVariable_Check(a[0]) && THPVariable_Check(a[1]) && THPVariable_Check(a[2]);
+        if (!ok) return false;
+        x = &THPVariable_Unpack(a[0]);
+        values = &THPVariable_Unpack(a[1]);
+        indices = &THPVariable_Unpack(a[2]);
+        rest = tensor_or_none(a[3], ok);
+        double t;
+        if (!ok || !number(a[4], t) || !usual_temperature(t)) return false;
+        int reduction;
+        if (text_is(a[5], "mean")) reduction = DDF_B200_MEAN;
+        else if (text_is(a[5], "sum")) reduction = DDF_B200_SUM;
+        else if (text_is(a[5], "none")) reduction = DDF_B200_NONE;
+        else return false;
+        Rows r;
+        if (!x->is_cuda() || !logits_dtype(*x) || !logits_dtype(*values) || !ordinary({x, values, indices}) || !r.of(*x)) return false;
+        const auto it = indices->scalar_type();
+        if (it != at::kLong && it != at::kInt) return false;
+        if (values->device() != x->device() || indices->device() != x->device()) return false;
+        if (!leading_is(*values, *x, 1) || values->sizes() != indices->sizes()) return false;
+        const int64_t k = values->size(-1);
+        if (k < 1 || k > 256 || !values->is_contiguous() || !indices->is_contiguous() || values->requires_grad()) return false;
+        if (rest && (!ordinary({rest}) || rest->device() != x->device() || rest->scalar_type() != at::kFloat || !leading_is(*rest, *x, 0) ||
+                     !rest->is_contiguous() || rest->requires_grad()))
+            return false;
+        args = ddf_b200_distill_args{};
+        args.rows = r.rows; args.classes = r.cols; args.row_stride = r.stride; args.k = (int)k;
+        args.dtype = dtype_code(x->scalar_type());
+        args.values_dtype = dtype_code(values->scalar_type());
+        args.wide_indices = it == at::kLong;
+        args.reduction = reduction;
+        args.temperature = t;
+        point(*x, *values, *indices, rest);
+        return true;
+    }
+    void point(const Tensor& l, const Tensor& v, const Tensor& i, const Tensor* r) {
+        args.logits = l.data_ptr();
+        args.values = v.data_ptr();
+        args.indices = i.data_ptr();
+        args.rest = r ? r->data_ptr<float>() : nullptr;
+    }
+};
+
+// What the forward leaves for the backward, in one tensor: stats, then the losses of a reduced loss, then the count.
+struct Scratch {
+    Tensor all;
+    float *stats, *losses;
+    int* count;
+    Scratch() = default;
+    Scratch(int64_t rows, const at::Device& dev)
+        : all(empty_like_on({rows * (DDF_B200_DISTILL_STATS + 1) + 1}, at::kFloat, dev)) { find(rows); }
+    void find(int64_t rows) {
+        stats = all.data_ptr<float>();
+        losses = stats + rows * DDF_B200_DISTILL_STATS;
+        count = reinterpret_cast<int*>(losses + rows);
+    }
+};
+
+struct DistillNode : public torch::autograd::Node {
+    std::string name() const override { return "DistillFunctionBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        x_.reset_data();
+        values_.reset_data();
+        indices_.reset_data();
+        rest_.reset_data();
+        scratch = Scratch();
+        released = true;
+    }
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+        torch::autograd::variable_list out(1);
+        std::lock_guard<std::mutex> lock(mutex_);
+        TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
+        if (!task_should_compute_output(0)) return out;
+        const Tensor x = x_.unpack(), values = values_.unpack(), indices = indices_.unpack(), rest = rest_.unpack();
+        at::NoGradGuard no_grad;
+        const at::Device dev = x.device();
+        c10::cuda::CUDAGuard on_device(dev);
+        Tensor up = grads[0];
+        // a gradient that never reached the output is zero, as torch.autograd.Function has it
+        if (!up.defined()) up = at::zeros({}, x.options().dtype(at::kFloat));
+        if (up.scalar_type() != at::kFloat) up = up.to(at::kFloat);
+        int64_t step = 0;
+        if (call.args.reduction == DDF_B200_NONE && up.numel() > 1) {
+            bool one = true;  // an expanded number
+            for (int64_t i = 0; i < up.dim(); ++i) one &= up.size(i) == 1 || up.stride(i) == 0;
+            if (!one) {
+                up = up.contiguous();
+                step = 1;
+            }
+        }
+        Tensor grad = empty_like_on(x.sizes(), x.scalar_type(), dev);
+        Distill c = call;
+        c.point(x, values, indices, rest.defined() ? &rest : nullptr);
+        check(lib.distill_backward(&c.args, scratch.stats, scratch.count, up.data_ptr<float>(), step, grad.data_ptr(), stream_of(dev)));
+        out[0] = grad;
+        return out;
+    }
+    Distill call;
+    Scratch scratch;
+    torch::autograd::SavedVariable x_, values_, indices_, rest_;
+    bool released = false;
+};
+
+PyObject* py_distill_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Distill c;
+    if (n != 6 || !c.parse(args)) Py_RETURN_NONE;
+    if (!loaded()) return nullptr;
+    const bool grad = at::GradMode::is_enabled() && c.x->requires_grad();
+    Tensor out;
+    {
+        pybind11::gil_scoped_release no_gil;
+        RECORD_FUNCTION("DistillFunction", std::vector<c10::IValue>({*c.x, *c.values, *c.indices}));
+        const at::Device dev = c.x->device();
+        c10::cuda::CUDAGuard on_device(dev);
+        const bool none = c.args.reduction == DDF_B200_NONE;
+        Scratch s(c.args.rows, dev);
+        out = empty_like_on(none ? leading(*c.x) : std::vector<int64_t>(), at::kFloat, dev);
+        float* o = out.data_ptr<float>();
+        check(lib.distill_forward(&c.args, none ? o : s.losses, s.stats, none ? nullptr : o, none ? nullptr : s.count, stream_of(dev)));
+        if (grad) {
+            std::shared_ptr<DistillNode> node(new DistillNode(), torch::autograd::deleteNode);
+            node->set_next_edges(torch::autograd::collect_next_edges(*c.x));
+            node->call = c;
+            node->scratch = s;
+            node->x_ = torch::autograd::SavedVariable(*c.x, false);
+            node->values_ = torch::autograd::SavedVariable(*c.values, false);
+            node->indices_ = torch::autograd::SavedVariable(*c.indices, false);
+            if (c.rest) node->rest_ = torch::autograd::SavedVariable(*c.rest, false);
+            torch::autograd::set_history(out, node);
+        }
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// ... and the loss's scale: loss and gradient
+PyObject* py_distill_loss_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Distill c;
+    double scale;
+    if (n != 7 || !c.parse(args) || !number(args[6], scale)) Py_RETURN_NONE;
+    if (!loaded()) return nullptr;
+    Tensor loss, grad;
+    {
+        pybind11::gil_scoped_release no_gil;
+        RECORD_FUNCTION("distill_loss_grad", std::vector<c10::IValue>({*c.x, *c.values, *c.indices}));
+        const at::Device dev = c.x->device();
+        c10::cuda::CUDAGuard on_device(dev);
+        const bool none = c.args.reduction == DDF_B200_NONE;
+        loss = empty_like_on(none ? leading(*c.x) : std::vector<int64_t>(), at::kFloat, dev);
+        grad = empty_like_on(c.x->sizes(), c.x->scalar_type(), dev);
+        Tensor scratch;
+        if (!none) scratch = empty_like_on({c.args.rows + DDF_B200_DISTILL_COUNTS}, at::kFloat, dev);
+        float* o = loss.data_ptr<float>();
+        int* counts = none ? nullptr : reinterpret_cast<int*>(scratch.data_ptr<float>() + c.args.rows);
+        check(lib.distill_loss_grad(&c.args, none ? o : scratch.data_ptr<float>(), counts, none ? nullptr : o, scale, grad.data_ptr(), stream_of(dev)));
+    }
+    PyObject* out = PyTuple_New(2);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(loss)));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(grad)));
+    return out;
+    END_HANDLE_TH_ERRORS
+}
+
+// ------------------------------------------------------------------ linear_act(x, weight, bias, residual, activation, add)
+struct LinearNode : public torch::autograd::Node {
+    std::string name() const override { return "LinearActFunctionBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        x_.reset_data();
+        w_.reset_data();
+        aux_.reset_data();
+        released = true;
+    }
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+        torch::autograd::variable_list out(4);
+        std::lock_guard<std::mutex> lock(mutex_);
+        TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
+        const Tensor x = x_.unpack(), w = w_.unpack(), aux = aux_.unpack(aux_is_output ? shared_from_this() : nullptr);
+        at::NoGradGuard no_grad;
+        const at::Device dev = x.device();
+        c10::cuda::CUDAGuard on_device(dev);
+        auto sizes = leading(x);
+        sizes.push_back(w.size(0));
+        // a gradient that never reached the output is zero, as torch.autograd.Function has it
+        Tensor gy = grads[0].defined() ? grads[0] : at::zeros(sizes, x.options());
+        if (gy.scalar_type() != x.scalar_type()) gy = gy.to(x.scalar_type());
+        Rows r;
+        if (!r.of(gy)) {
+            gy = gy.contiguous();
+            r.of(gy);
+        }
+        // a residual behind the activation, or of a call without one, has the gradient that arrives
+        const bool through = args.after || args.activation == DDF_B200_ACT_NONE;
+        const bool need_r = task_should_compute_output(3);
+        Tensor gx, gw, gb, gr;
+        if (task_should_compute_output(0)) gx = empty_like_on(x.sizes(), x.scalar_type(), dev);
+        if (task_should_compute_output(1)) gw = empty_like_on(w.sizes(), x.scalar_type(), dev);
+        if (task_should_compute_output(2)) gb = empty_like_on({w.size(0)}, x.scalar_type(), dev);
+        if (need_r && !through) gr = empty_like_on(sizes, x.scalar_type(), dev);
+        if (gx.defined() || gw.defined() || gb.defined() || gr.defined()) {
+            ddf_b200_linear_args a = args;
+            a.x = x.data_ptr();
+            a.weight = w.data_ptr();
+            a.bias = a.residual = nullptr;
+            const size_t bytes = lib.linear_backward_workspace(&a, gy.data_ptr(), r.stride, ptr(gx), ptr(gw), ptr(gb), ptr(gr));
+            Tensor ws;
+            if (bytes) ws = empty_like_on({(int64_t)bytes}, at::kByte, dev);
+            check(lib.linear_backward(&a, gy.data_ptr(), r.stride, ptr(aux), ptr(gx), ptr(gw), ptr(gb), ptr(gr), ptr(ws), bytes, stream_of(dev)));
+        }
+        out[0] = gx;
+        out[1] = gw;
+        out[2] = gb;
+        out[3] = need_r && through ? gy : gr;
+        return out;
+    }
+    ddf_b200_linear_args args;
+    torch::autograd::SavedVariable x_, w_, aux_;
+    bool aux_is_output = false, released = false;
+};
+
+PyObject* py_linear_act(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6 || !THPVariable_Check(a[0]) || !THPVariable_Check(a[1])) Py_RETURN_NONE;
+    bool ok = true;
+    const Tensor *x = &THPVariable_Unpack(a[0]), *w = &THPVariable_Unpack(a[1]), *b = tensor_or_none(a[2], ok), *res = tensor_or_none(a[3], ok);
+    ddf_b200_linear_args q{};
+    if (text_is(a[4], "none")) q.activation = DDF_B200_ACT_NONE;
+    else if (text_is(a[4], "relu")) q.activation = DDF_B200_ACT_RELU;
+    else if (text_is(a[4], "gelu")) q.activation = DDF_B200_ACT_GELU;
+    else if (text_is(a[4], "silu")) q.activation = DDF_B200_ACT_SILU;
+    else ok = false;
+    if (text_is(a[5], "after")) q.after = 1;
+    else if (!text_is(a[5], "before")) ok = false;
+    const auto dt = x->scalar_type();
+    Rows xr, wr, rr;
+    if (!ok || !x->is_cuda() || (dt != at::kHalf && dt != at::kBFloat16) || at::autocast::is_autocast_enabled(at::kCUDA) || !ordinary({x, w}) ||
+        w->scalar_type() != dt || w->device() != x->device() || w->dim() != 2 || !xr.of(*x) || !wr.of(*w) || xr.cols != wr.cols)
+        Py_RETURN_NONE;
+    const int64_t outputs = wr.rows;
+    if (b && (!ordinary({b}) || b->scalar_type() != dt || b->device() != x->device() || b->dim() != 1 || b->size(0) != outputs || !b->is_contiguous()))
+        Py_RETURN_NONE;
+    if (res && (!ordinary({res}) || res->scalar_type() != dt || res->device() != x->device() || !leading_is(*res, *x, 1) || res->size(-1) != outputs || !rr.of(*res)))
+        Py_RETURN_NONE;
+    if (!loaded()) return nullptr;
+    const auto wants = [](const Tensor* t) { return t && t->requires_grad(); };
+    const bool grad = at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b) || wants(res));
+    Tensor y;
+    {
+        pybind11::gil_scoped_release no_gil;
+        RECORD_FUNCTION("LinearActFunction", std::vector<c10::IValue>({*x, *w}));
+        const at::Device dev = x->device();
+        c10::cuda::CUDAGuard on_device(dev);
+        auto sizes = leading(*x);
+        sizes.push_back(outputs);
+        y = empty_like_on(sizes, dt, dev);
+        // what the activation's slope is taken at: its input, or, where a ReLU ends the call, its output
+        Tensor aux;
+        const bool relu = q.activation == DDF_B200_ACT_RELU && !(q.after && res);
+        if (grad && q.activation != DDF_B200_ACT_NONE && !relu) aux = empty_like_on(sizes, dt, dev);
+        q.x = x->data_ptr();
+        q.weight = w->data_ptr();
+        q.bias = b ? b->data_ptr() : nullptr;
+        q.residual = res ? res->data_ptr() : nullptr;
+        q.rows = xr.rows; q.inputs = xr.cols; q.outputs = outputs;
+        q.x_stride = xr.stride; q.weight_stride = wr.stride; q.residual_stride = rr.stride;
+        q.dtype = dtype_code(dt);
+        const size_t bytes = lib.linear_workspace(&q);
+        Tensor ws;
+        if (bytes) ws = empty_like_on({(int64_t)bytes}, at::kByte, dev);
+        check(lib.linear_forward(&q, y.data_ptr(), ptr(aux), ptr(ws), bytes, stream_of(dev)));
+        if (grad) {
+            std::shared_ptr<LinearNode> node(new LinearNode(), torch::autograd::deleteNode);
+            static const Tensor nothing;
+            node->set_next_edges(torch::autograd::collect_next_edges(*x, *w, b ? *b : nothing, res ? *res : nothing));
+            node->args = q;
+            node->x_ = torch::autograd::SavedVariable(*x, false);
+            node->w_ = torch::autograd::SavedVariable(*w, false);
+            torch::autograd::set_history(y, node);
+            node->aux_is_output = relu;
+            if (relu) node->aux_ = torch::autograd::SavedVariable(y, true);
+            else if (aux.defined()) node->aux_ = torch::autograd::SavedVariable(aux, false);
+        }
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef functions[] = {
+    {"top_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_top_logits)), METH_FASTCALL,
+     "top_logits(logits, k, temperature) -> (values, indices, rest), or None"},
+    {"distill_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_distill_loss)), METH_FASTCALL,
+     "distill_loss(logits, values, indices, rest, temperature, reduction) -> the loss, or None"},
+    {"distill_loss_grad", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_distill_loss_grad)), METH_FASTCALL,
+     "distill_loss_grad(logits, values, indices, rest, temperature, reduction, scale) -> (loss, gradient), or None"},
+    {"linear_act", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_act)), METH_FASTCALL,
+     "linear_act(x, weight, bias, residual, activation, add) -> the output, or None"},
+    {nullptr, nullptr, 0, nullptr}};
+
+}  // namespace
+
+bool add_head(PyObject* module) { return PyModule_AddFunctions(module, functions) == 0; }
+
+}  // namespace ddf_native

@@ -9,6 +9,8 @@
 The mathematics stands in include/ddf_b200.h and csrc/distill.cu.  Logits are float32, float16 or bfloat16 CUDA
 tensors of any leading shape whose last dimension is the classes; sums and losses are float32.  Rows may lie any
 number of elements apart; other layouts are copied first.  There is no CPU path.
+
+Ordinary calls run through csrc/native_head.cpp; it leaves every other one to the functions here.
 """
 from __future__ import annotations
 
@@ -19,7 +21,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from . import _lib
+from . import _lib, op
 
 _DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _REDUCTIONS = {"none": _lib.NONE, "sum": _lib.SUM, "mean": _lib.MEAN}
@@ -64,6 +66,10 @@ def _row_stride(flat):
 def top_logits(logits, k, temperature=1.0):
     """The k (at most 256) largest ``logits`` of each row in descending order, equal ones by ascending class and
     NaN above all numbers; and the log of the others' sum of ``exp(logit / temperature)``.  Records no gradient."""
+    if op._native is not None or op._import_native():
+        top = op._native.top_logits(logits, k, temperature)
+        if top is not None:
+            return TopLogits(*top)
     _check_logits(logits, "logits")
     temperature = _check_temperature(temperature)
     classes, k = logits.shape[-1], int(k)
@@ -168,6 +174,10 @@ def distill_loss(logits, values, indices, rest=None, temperature=1.0, reduction=
     Without ``rest`` the teacher's softmax is over its listed classes alone.  An index outside the classes is an
     empty entry; a row of nothing else does not count (loss and gradient 0, left out of the mean).  Returns a
     float32 scalar, or, with ``reduction='none'``, one loss a row; the gradient goes to ``logits`` alone."""
+    if op._native is not None or op._import_native():
+        loss = op._native.distill_loss(logits, values, indices, rest, temperature, reduction)
+        if loss is not None:
+            return loss
     _check_targets(logits, values, indices, rest, reduction)
     return DistillFunction.apply(logits, values, indices, rest, _check_temperature(temperature), reduction)
 
@@ -176,6 +186,10 @@ def distill_loss_grad(logits, values, indices, rest=None, temperature=1.0, reduc
     """``(loss, gradient)``: what ``distill_loss`` returns, and ``scale`` times its gradient with respect to
     ``logits`` (with ``reduction='none'``: that of the losses' sum), contiguous and of their type.  Reads the logits
     once.  Records no autograd history."""
+    if op._native is not None or op._import_native():
+        both = op._native.distill_loss_grad(logits, values, indices, rest, temperature, reduction, scale)
+        if both is not None:
+            return both
     _check_targets(logits, values, indices, rest, reduction)
     temperature = _check_temperature(temperature)
     lead, dev = logits.shape[:-1], logits.device

@@ -3,7 +3,7 @@ tensor cores (csrc/linear.cuh).  What a classifier and the 1x1 convolutions of a
 ``x.permute(0, 2, 3, 1)`` of a channels_last tensor has a row for each pixel.
 
 float16 and bfloat16 CUDA tensors, all of one type; sums are float, results are rounded once.  Under autocast the
-arguments are cast to its type.  There is no CPU path.
+arguments are cast to its type.  There is no CPU path.  Ordinary calls run through csrc/native_head.cpp.
 """
 from __future__ import annotations
 
@@ -13,7 +13,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from . import _lib
+from . import _lib, op
 from .distill import _row_stride, _rows
 
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -120,6 +120,10 @@ def linear_act(x, weight, bias=None, residual=None, activation="none", add="befo
     ``x`` (..., inputs), ``weight`` (outputs, inputs), ``bias`` (outputs), ``residual`` (..., outputs);
     ``activation`` 'none', 'relu', 'gelu' (by erf) or 'silu'.  Rows may lie any number of elements apart.  Gradients go
     to every tensor; the activation's input is kept for them in the tensors' type."""
+    if op._native is not None or op._import_native():
+        y = op._native.linear_act(x, weight, bias, residual, activation, add)
+        if y is not None:
+            return y
     if torch.is_autocast_enabled("cuda") and x.is_cuda:
         dt = torch.get_autocast_dtype("cuda")
         x, weight, bias, residual = (t.to(dt) if t is not None and t.is_floating_point() else t

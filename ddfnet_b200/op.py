@@ -286,7 +286,10 @@ def _bind_native():
     """Hands the library's entry points to the native module (the first call does this)."""
     lib = _lib.load()
     names = ("ddf_b200_forward", "ddf_b200_forward_sfnorm", "ddf_b200_backward_workspace", "ddf_b200_backward",
-             "ddf_b200_sfnorm", "ddf_b200_sfnorm_backward", "ddf_b200_take_fault", "ddf_b200_maxpool_nhwc")
+             "ddf_b200_sfnorm", "ddf_b200_sfnorm_backward", "ddf_b200_take_fault", "ddf_b200_maxpool_nhwc",
+             "ddf_b200_top_logits", "ddf_b200_distill_forward", "ddf_b200_distill_backward",
+             "ddf_b200_distill_loss_grad", "ddf_b200_linear_workspace", "ddf_b200_linear_forward",
+             "ddf_b200_linear_backward_workspace", "ddf_b200_linear_backward")
     _native.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}, _lib._DEBUG)
 
 
