@@ -112,9 +112,9 @@ struct BackPlan {
     void *gz, *gz2;    // either may be NULL; rows ldz / N apart
     float* sums;       // chunks x N, or NULL
     long long ldg, ldz, M;
-    int N, act, chunk, vec, vecz;
+    int N, chunk, vec, vecz;
 };
-template <typename T> __global__ void __launch_bounds__(256) linear_back_kernel(const BackPlan p) {
+template <typename T, int ACT> __global__ void __launch_bounds__(256) linear_back_kernel(const BackPlan p) {
     __shared__ float4 sums[8][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.x * 128 + lane * 4, left = p.N - col;
@@ -125,10 +125,10 @@ template <typename T> __global__ void __launch_bounds__(256) linear_back_kernel(
         for (long long r = r0 + warp; r < r1; r += 8) {
             float g[4], z[4];
             load4(reinterpret_cast<const T*>(p.gy) + r * p.ldg + col, p.vec, left, g);
-            if (p.act != kActNone) {
+            if constexpr (ACT != kActNone) {
                 load4(reinterpret_cast<const T*>(p.aux) + r * p.N + col, p.vec, left, z);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) g[i] *= act_slope(z[i], p.act);
+                for (int i = 0; i < 4; ++i) g[i] *= act_slope<ACT>(z[i]);
             }
             if (p.gz) store4(reinterpret_cast<T*>(p.gz) + r * p.ldz + col, p.vecz, left, g);
             if (p.gz2) store4(reinterpret_cast<T*>(p.gz2) + r * p.N + col, p.vec, left, g);
@@ -230,6 +230,15 @@ static Cut cut_of(long long M, long long N, long long K, int sm_count) {
 }
 static size_t partial_bytes(long long M, long long N, const Cut& c) { return c.splits > 1 ? (size_t)c.splits * M * N * 4 : 0; }
 
+template <typename T, bool AT, bool BT> static auto kernel_of(int bn, int act) {
+    if constexpr (!AT && !BT) {
+        if (act == kActRelu) return bn == 256 ? linear_kernel<T, 256, AT, BT, kActRelu> : bn == 128 ? linear_kernel<T, 128, AT, BT, kActRelu> : linear_kernel<T, 64, AT, BT, kActRelu>;
+        if (act == kActGelu) return bn == 256 ? linear_kernel<T, 256, AT, BT, kActGelu> : bn == 128 ? linear_kernel<T, 128, AT, BT, kActGelu> : linear_kernel<T, 64, AT, BT, kActGelu>;
+        if (act == kActSilu) return bn == 256 ? linear_kernel<T, 256, AT, BT, kActSilu> : bn == 128 ? linear_kernel<T, 128, AT, BT, kActSilu> : linear_kernel<T, 64, AT, BT, kActSilu>;
+    }
+    return bn == 256 ? linear_kernel<T, 256, AT, BT, kActNone> : bn == 128 ? linear_kernel<T, 128, AT, BT, kActNone> : linear_kernel<T, 64, AT, BT, kActNone>;
+}
+
 // D (M x N) = A B^T.  at / bt: the matrix given is stored with the reduction as its rows.
 template <typename T, bool AT, bool BT>
 static int product(const Matrix& a, const Matrix& b, long long M, long long N, long long K, const Epilogue& out, float* partial, int dtype, long long limit,
@@ -238,7 +247,7 @@ static int product(const Matrix& a, const Matrix& b, long long M, long long N, l
     int rc = device_facts(&sm, &fault, &index);
     if (rc) return rc;
     const Cut cut = cut_of(M, N, K, sm);
-    auto kernel = cut.bn == 256 ? linear_kernel<T, 256, AT, BT> : cut.bn == 128 ? linear_kernel<T, 128, AT, BT> : linear_kernel<T, 64, AT, BT>;
+    auto kernel = kernel_of<T, AT, BT>(cut.bn, cut.splits > 1 ? (int)kActNone : out.act);  // (splits finish in the join)
     // (before the driver's encoder: a runtime call gives a thread that has none its context)
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinearShared);
     if (e != cudaSuccess) return (int)e;
@@ -370,10 +379,12 @@ static int backward(const ddf_b200_linear_args* q, const void* gy, long long gy_
 
     int rc;
     if (scratch || want_gr || gb) {
-        BackPlan b{gy, aux, scratch ? gzp : nullptr, want_gr ? gr : nullptr, sums, gy_stride, padded(N), M, (int)N, q->activation, (int)chunk, 0, 0};
+        BackPlan b{gy, aux, scratch ? gzp : nullptr, want_gr ? gr : nullptr, sums, gy_stride, padded(N), M, (int)N, (int)chunk, 0, 0};
         b.vec = by_four(gy, gy_stride) && (!act || by_four(aux, N)) && (!want_gr || by_four(gr, N));
         b.vecz = 1;
-        linear_back_kernel<T><<<dim3((unsigned)((N + 127) / 128), (unsigned)chunks), 256, 0, st>>>(b);
+        auto kernel = q->activation == kActRelu ? linear_back_kernel<T, kActRelu> : q->activation == kActGelu ? linear_back_kernel<T, kActGelu>
+                      : q->activation == kActSilu ? linear_back_kernel<T, kActSilu> : linear_back_kernel<T, kActNone>;
+        kernel<<<dim3((unsigned)((N + 127) / 128), (unsigned)chunks), 256, 0, st>>>(b);
         if ((rc = launched())) return rc;
         if (gb) {
             linear_bias_kernel<T><<<(unsigned)((N + 31) / 32), 256, 0, st>>>(sums, (T*)gb, (int)chunks, (int)N);
