@@ -190,45 +190,52 @@ struct Matrix {
 static bool addressable(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 static long long padded(long long n) { return (n + 7) / 8 * 8; }
 
-static int encode(CUtensorMap* map, const Matrix& m, int dtype, int box_rows) {
+static int encode(CUtensorMap* map, CUtensorMapDataType type, const void* at, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                  CUtensorMapSwizzle swizzle) {
     const EncodeTiled f = encode_tiled();
     if (!f) return DDF_B200_E_DEVICE;
+    const cuuint32_t unit[3] = {1, 1, 1};
+    return f(map, type, (cuuint32_t)rank, const_cast<void*>(at), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : DDF_B200_E_ARGUMENT;
+}
+// Boxes of box_cols x box_rows of a 2-byte matrix.
+static int encode_matrix(CUtensorMap* map, const Matrix& m, int dtype, int box_cols, int box_rows) {
     const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.ld * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, unit[2] = {1, 1};
-    return f(map, dtype == DDF_B200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(m.p), dims, strides, box,
-             unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : DDF_B200_E_ARGUMENT;
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+    return encode(map, dtype == DDF_B200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, m.p, 2, dims, strides, box,
+                  box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// How a product is cut: columns of a tile and splits of K.
+// How a product is cut: columns of a tile, splits of K, and whether a cluster of blocks joins them.
 struct Cut {
     int bn, splits, steps;
+    bool cluster;
 };
 static Cut cut_of(long long M, long long N, long long K, int sm_count) {
     const long long steps = (K + kTileK - 1) / kTileK, tiles_m = (M + kTileM - 1) / kTileM;
-    Cut best{256, 1, (int)steps};
+    Cut best{256, 1, (int)steps, false};
     double least = 1e300;
     for (int bn : {256, 128, 64}) {
         if (bn > 64 && N <= bn / 2) continue;
         // clocks of a step of 64 along K, and of a tile's start and end
         const double step = bn == 256 ? 600 : bn == 128 ? 370 : 260, once = 1200 + 5 * bn;
         const long long tiles = tiles_m * ((N + bn - 1) / bn);
-        for (int want = 1; want <= 32; ++want) {
+        for (int want : {1, 2, 4, 8, 12, 16, 24, 32, 48}) {
             const long long per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
-            if (splits != want) continue;
-            if (splits > 1 && (per < 4 || (double)splits * M * N > 64e6)) break;
+            if (splits > 1 && (per < 2 || (splits > 8 && (double)splits * M * N > 64e6))) break;
+            const bool cluster = splits > 1 && splits <= 8 && bn <= 128;
             const long long waves = (tiles * splits + sm_count - 1) / sm_count;
-            const double join = splits > 1 ? 4000 + (double)M * N * (8 * splits + 4) / 3000 : 0;
-            const double cost = (double)waves * (per * step + once) + join;
+            const double join = cluster ? 1500 : splits > 1 ? 4000 + (double)M * N * (8 * splits + 4) / 3000 : 0;
+            const double cost = (double)waves * (per * step + once + (cluster ? join : 0)) + (cluster ? 0 : join);
             if (cost < least * 0.97) {
                 least = cost;
-                best = Cut{bn, (int)splits, (int)per};
+                best = Cut{bn, (int)splits, (int)per, cluster};
             }
         }
     }
     return best;
 }
-static size_t partial_bytes(long long M, long long N, const Cut& c) { return c.splits > 1 ? (size_t)c.splits * M * N * 4 : 0; }
+static size_t partial_bytes(long long M, long long N, const Cut& c) { return c.splits > 1 && !c.cluster ? (size_t)c.splits * M * N * 4 : 0; }
 
 template <typename T, bool AT, bool BT> static auto kernel_of(int bn, int act) {
     if constexpr (!AT && !BT) {
@@ -247,29 +254,57 @@ static int product(const Matrix& a, const Matrix& b, long long M, long long N, l
     int rc = device_facts(&sm, &fault, &index);
     if (rc) return rc;
     const Cut cut = cut_of(M, N, K, sm);
-    auto kernel = kernel_of<T, AT, BT>(cut.bn, cut.splits > 1 ? (int)kActNone : out.act);  // (splits finish in the join)
+    const bool joined = cut.splits > 1 && !cut.cluster;  // by a kernel of its own, which finishes too
+    auto kernel = kernel_of<T, AT, BT>(cut.bn, joined ? (int)kActNone : out.act);
     // (before the driver's encoder: a runtime call gives a thread that has none its context)
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinearShared);
     if (e != cudaSuccess) return (int)e;
     LinearPlan p{};
-    if ((rc = encode(&p.a, a, dtype, AT ? kTileK : kTileM))) return rc;
-    if ((rc = encode(&p.b, b, dtype, BT ? kTileK : cut.bn))) return rc;
+    if ((rc = encode_matrix(&p.a, a, dtype, 64, AT ? kTileK : kTileM))) return rc;
+    if ((rc = encode_matrix(&p.b, b, dtype, 64, BT ? kTileK : cut.bn))) return rc;
     p.out = out;
-    p.partial = cut.splits > 1 ? partial : nullptr;
+    if (joined) {
+        p.partial = partial;
+        p.boxes = N % 4 == 0;
+        const cuuint64_t dims[3] = {(cuuint64_t)N, (cuuint64_t)M, (cuuint64_t)cut.splits}, strides[2] = {(cuuint64_t)N * 4, (cuuint64_t)M * N * 4};
+        const cuuint32_t box[3] = {32, 32, 1};
+        if (p.boxes && (rc = encode(&p.y, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, partial, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+    } else {
+        p.boxes = addressable(out.y, out.ldy) && (!out.aux || addressable(out.aux, out.ldy)) && (!out.residual || addressable(out.residual, out.ldr));
+        p.bias_vec = (reinterpret_cast<uintptr_t>(out.bias) & 15) == 0;
+        if (p.boxes) {
+            if ((rc = encode_matrix(&p.y, Matrix{out.y, M, N, out.ldy}, dtype, 32, 32))) return rc;
+            if (out.aux && (rc = encode_matrix(&p.aux, Matrix{out.aux, M, N, out.ldy}, dtype, 32, 32))) return rc;
+            if (out.residual && (rc = encode_matrix(&p.r, Matrix{out.residual, M, N, out.ldr}, dtype, 32, 32))) return rc;
+        }
+    }
     p.M = (int)M; p.N = (int)N; p.K = (int)K;
     p.tiles_m = (int)((M + kTileM - 1) / kTileM);
     p.tiles_n = (int)((N + cut.bn - 1) / cut.bn);
     p.splits = cut.splits;
     p.steps = cut.steps;
+    p.cluster = cut.cluster ? cut.splits : 1;
     const uint32_t type = dtype == DDF_B200_BF16 ? 1u : 0u;
     p.idesc = 1u << 4 | type << 7 | type << 10 | (AT ? 1u << 15 : 0u) | (BT ? 1u << 16 : 0u) | (uint32_t)(cut.bn / 8) << 17 | (uint32_t)(kTileM / 16) << 24;
     p.fault = fault;
     p.limit = limit;
     const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
     if (items > 0x7fffffffll) return DDF_B200_E_TOO_LARGE;
-    kernel<<<(unsigned)(items < sm ? items : sm), kLinearThreads, kLinearShared, st>>>(p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(cut.cluster || items < sm ? items : sm));
+    cfg.blockDim = dim3(kLinearThreads);
+    cfg.dynamicSmemBytes = kLinearShared;
+    cfg.stream = st;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)p.cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = cut.cluster ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kernel, p);
+    if (e != cudaSuccess) return (int)e;
     rc = launched();
-    if (rc || cut.splits == 1) return rc;
+    if (rc || !joined) return rc;
     linear_join_kernel<T><<<(unsigned)((M * ((N + 3) / 4) + 255) / 256), 256, 0, st>>>(partial, out, (int)M, (int)N, cut.splits);
     return launched();
 }

@@ -11,11 +11,12 @@
 // results' bytes.  One persistent block an SM:
 //   warp 0     one thread loads tiles of 64 along K by TMA into a ring of stages (192 KB)
 //   warp 1     one thread issues the products, 128 x BN, into one of two accumulators in tensor memory
-//   warps 4-11 take the other accumulator meanwhile: 32 x 32 pieces through shared memory, so that eight
-//              lanes read and write 64 bytes of one row
+//   warps 4-11 take the other accumulator meanwhile, in pieces of 32 x 32: a thread holds a row of it; residual and
+//              results pass through shared memory to and from TMA, whose copies the warp does not wait for
 // BN = 256 where the tiles fill the machine: a 128 x 256 tile's operands take 96 bytes of shared memory a clock
-// at the full rate, a 128 x 128 tile's all 128.  Smaller BN and splits of K (partial sums in the workspace, joined
-// in a fixed order by linear_join_kernel) where they would not.
+// at the full rate, a 128 x 128 tile's all 128.  Where they would not, smaller BN and splits of K: up to eight
+// blocks of a cluster take one tile, and join its pieces out of each other's shared memory, in the order of K; more
+// splits leave partial sums in the workspace, joined in that order by linear_join_kernel.
 //
 // Every wait is bounded: a role whose wait runs out records a fault and leaves its loop, the others follow by their
 // own limits; the block meets after a pause in which its copies land, frees the tensor memory and ends.
@@ -30,7 +31,7 @@ constexpr int kTileM = 128, kTileK = 64;
 constexpr int kLinearThreads = 384, kJoinWarps = 8;
 constexpr uint32_t kRingBytes = 192 * 1024;
 constexpr uint32_t kPieceBytes = 32 * 32 * 4;  // an epilogue warp's piece
-constexpr uint32_t kLinearShared = kRingBytes + kJoinWarps * kPieceBytes + 1024 + 256;
+constexpr uint32_t kLinearShared = kRingBytes + kJoinWarps * kPieceBytes + 1024 + 512;
 
 enum Act { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
 
@@ -138,30 +139,160 @@ __device__ __forceinline__ void finish4(const Epilogue& e, long long row, int co
 
 struct LinearPlan {
     CUtensorMap a, b;
+    CUtensorMap y, aux, r;  // outputs (y: or the partial sums) and residual, where `boxes`
     Epilogue out;
-    float* partial;      // splits x M x N, where splits > 1
+    float* partial;         // splits x M x N, where the workspace joins them
     int M, N, K;
     int tiles_m, tiles_n, splits, steps;  // steps of 64 along K in a split
+    int cluster;            // blocks that share a tile, each with its split
+    int boxes;              // TMA can address the outputs and the residual
+    int bias_vec;           // ... and 16-byte loads the bias
     uint32_t idesc;
     int* fault;
-    long long limit;     // of a wait, in clocks
+    long long limit;        // of a wait, in clocks
 };
 
 // Work item -> tile and split: tiles of eight blocks of rows side by side, so that the tiles in flight share operands.
 __device__ __forceinline__ void tile_of(const LinearPlan& p, int item, int& m, int& n, int& split) {
     const int tiles = p.tiles_m * p.tiles_n;
-    split = item / tiles;
-    const int t = item - split * tiles;
+    int t;
+    if (p.cluster > 1) {
+        t = item / p.cluster;
+        split = item - t * p.cluster;
+    } else {
+        split = item / tiles;
+        t = item - split * tiles;
+    }
     const int group = t / (8 * p.tiles_n), in = t - group * 8 * p.tiles_n;
     const int rows = min(8, p.tiles_m - group * 8);
     m = group * 8 + in % rows;
     n = in / rows;
 }
 
+// What an epilogue warp needs to finish a piece of 32 rows x 32 columns, one row a lane.
+struct Piece {
+    uint32_t stage;   // 4 KB: results, then (from 2 KB on) the residual; or floats
+    uint32_t bar;     // of the residual's copy
+    uint32_t phase;
+    bool late;
+};
+// 16-byte unit u of row `lane` of a box of 64-byte rows (64-byte swizzle) or 128-byte rows (128-byte swizzle).
+__device__ __forceinline__ uint32_t unit64(int lane, int u) { return lane * 64 + ((u ^ (lane >> 1 & 3)) * 16); }
+__device__ __forceinline__ uint32_t unit128(int lane, int u) { return lane * 128 + ((u ^ (lane & 7)) * 16); }
+
+__device__ __forceinline__ void fetch_residual(const LinearPlan& p, const Piece& w, int row0, int col, int lane) {
+    if (lane == 0) {
+        mbar_arrive_expect_tx(w.bar, 2048);
+        tma_load_2d(w.stage + 2048, &p.r, col, row0, w.bar);
+    }
+}
+
+// `next`: called when the residual of this piece is in registers.  v: the lane's row of the product.
+template <typename T, int ACT, typename Next>
+__device__ __forceinline__ void finish_piece(const LinearPlan& p, Piece& w, float (&z)[32], int row0, int col, int split, int lane, Next next) {
+    const Epilogue& e = p.out;
+    if (p.partial) {
+        if (p.boxes) {
+            if (lane == 0) tma_store_wait_read();
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                sts128(w.stage + unit128(lane, u), __float_as_uint(z[4 * u]), __float_as_uint(z[4 * u + 1]), __float_as_uint(z[4 * u + 2]), __float_as_uint(z[4 * u + 3]));
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_3d(&p.y, w.stage, col, row0, split);
+                tma_store_commit();
+            }
+            return;
+        }
+    } else if (p.boxes) {
+        if (e.bias) {
+            const T* bias = reinterpret_cast<const T*>(e.bias) + col;
+            if (p.bias_vec && col + 32 <= p.N) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const uint4 g = __ldg(reinterpret_cast<const uint4*>(bias) + u);
+                    const uint32_t q[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) z[8 * u + i] += Word<T>::get(q[i / 2], i % 2);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (col + i < p.N) z[i] += Elem<T>::load(bias + i);
+            }
+        }
+        uint32_t r[16];
+        if (e.residual) {
+            if (!w.late && !mbar_wait_for(w.bar, w.phase, p.limit)) w.late = true;
+            w.phase ^= 1u;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) lds128v(w.stage + 2048 + unit64(lane, u), r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
+            fence_async();  // these reads come before the next copy's writes: the warp's barrier alone does not see to that
+            __syncwarp();
+            next();
+        }
+        const auto add = [&] {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] += Word<T>::get(r[i / 2], i % 2);
+        };
+        const auto store = [&](const CUtensorMap* map) {
+            if (lane == 0) tma_store_wait_read();
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                sts128(w.stage + unit64(lane, u), Word<T>::put(z[8 * u], z[8 * u + 1]), Word<T>::put(z[8 * u + 2], z[8 * u + 3]),
+                       Word<T>::put(z[8 * u + 4], z[8 * u + 5]), Word<T>::put(z[8 * u + 6], z[8 * u + 7]));
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d(map, w.stage, col, row0);
+                tma_store_commit();
+            }
+        };
+        if (e.residual && !e.after) add();
+        if (e.aux) store(&p.aux);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z[i] = act_value<ACT>(z[i]);
+        if (e.residual && e.after) add();
+        store(&p.y);
+        return;
+    }
+    // rows that TMA cannot address: turned in shared memory, a column a lane
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+        sts128(w.stage + unit128(lane, u), __float_as_uint(z[4 * u]), __float_as_uint(z[4 * u + 1]), __float_as_uint(z[4 * u + 2]), __float_as_uint(z[4 * u + 3]));
+    __syncwarp();
+    const int c = col + lane, rows = min(32, p.M - row0);
+    if (c < p.N) {
+        const float bias = !p.partial && e.bias ? Elem<T>::load(reinterpret_cast<const T*>(e.bias) + c) : 0.f;
+#pragma unroll 4
+        for (int i = 0; i < rows; ++i) {
+            const long long row = row0 + i;
+            float v = ldsf(w.stage + unit128(i, lane >> 2) + (lane & 3) * 4);
+            if (p.partial) {
+                p.partial[((long long)split * p.M + row) * p.N + c] = v;
+            } else {
+                const float r = e.residual ? Elem<T>::load(reinterpret_cast<const T*>(e.residual) + row * e.ldr + c) : 0.f;
+                v += bias;
+                if (!e.after) v += r;
+                if (e.aux) Elem<T>::store(reinterpret_cast<T*>(e.aux) + row * e.ldy + c, v);
+                v = act_value<ACT>(v);
+                if (e.after) v += r;
+                Elem<T>::store(reinterpret_cast<T*>(e.y) + row * e.ldy + c, v);
+            }
+        }
+    }
+    __syncwarp();
+}
+
 template <typename T, int BN, bool AT, bool BT, int ACT>
 __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_constant__ LinearPlan p) {
     constexpr uint32_t kA = kTileM * kTileK * 2, kB = BN * kTileK * 2, kStage = kA + kB;
     constexpr int kStages = (int)(kRingBytes / kStage);
+    constexpr int kSlots = 4 * (BN / 32);  // pieces of a tile
+    constexpr bool kJoins = 2 * kSlots * kPieceBytes <= kRingBytes;  // a tile's sums, sent and received, fit the ring
     extern __shared__ unsigned char linear_raw[];
     const uint32_t base = (smem_u32(linear_raw) + 1023u) & ~1023u;
     const uint32_t pieces = base + kRingBytes, bars = pieces + kJoinWarps * kPieceBytes;
@@ -169,7 +300,9 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
     const auto empty = [&](int s) { return bars + 8u * (kStages + s); };
     const auto acc_full = [&](int s) { return bars + 8u * (2 * kStages + s); };
     const auto acc_empty = [&](int s) { return bars + 8u * (2 * kStages + 2 + s); };
-    const uint32_t tmem_word = bars + 8u * (2 * kStages + 4);
+    const auto res_bar = [&](int w) { return bars + 8u * (2 * kStages + 4 + w); };
+    const auto join_bar = [&](int w) { return bars + 8u * (2 * kStages + 4 + kJoinWarps + w); };
+    const uint32_t tmem_word = bars + 8u * (2 * kStages + 4 + 2 * kJoinWarps);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int items = p.tiles_m * p.tiles_n * p.splits;
     const int all_steps = (p.K + kTileK - 1) / kTileK;
@@ -184,9 +317,11 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
             mbar_init(acc_full(s), 1);
             mbar_init(acc_empty(s), kJoinWarps);
         }
+        for (int w = 0; w < 2 * kJoinWarps; ++w) mbar_init(res_bar(w), 1);  // (join_bar too)
         mbar_fence_init();
         tma_prefetch_map(&p.a);
         tma_prefetch_map(&p.b);
+        if (p.boxes) tma_prefetch_map(&p.y);
     }
     if (warp == 2) tmem_alloc(tmem_word, 2 * BN);
     tc_fence_before();
@@ -251,112 +386,113 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
         }
     } else if (warp >= 4) {
         const int quarter = warp & 3, half = (warp - 4) >> 2;
-        const uint32_t piece = pieces + (uint32_t)(warp - 4) * kPieceBytes;
-        const int sub = lane & 7;  // four columns of a piece
+        const int c0 = half * (BN / 2), c1 = c0 + BN / 2;
+        Piece w{pieces + (uint32_t)(warp - 4) * kPieceBytes, res_bar(warp - 4), 0u, false};
+        const bool residual = p.out.residual && p.boxes && !p.partial;
         int acc = 0;
         uint32_t acc_phase = 0;
+        int m = 0, n = 0, split = 0;
+        if (blockIdx.x < items) tile_of(p, blockIdx.x, m, n, split);
+        if (residual && p.cluster == 1 && blockIdx.x < items) fetch_residual(p, w, m * kTileM + quarter * 32, n * BN + c0, lane);
         for (int item = blockIdx.x; item < items; item += gridDim.x) {
-            int m, n, split;
-            tile_of(p, item, m, n, split);
+            int m2 = 0, n2 = 0, split2 = 0;
+            const bool more = item + (int)gridDim.x < items;
+            if (more) tile_of(p, item + gridDim.x, m2, n2, split2);
             if (!mbar_wait_for(acc_full(acc), acc_phase, p.limit)) { late = true; break; }
             tc_fence_after();
-            const int row0 = m * kTileM + quarter * 32 + (lane >> 3);
-            const bool whole = m * kTileM + kTileM <= p.M && n * BN + BN <= p.N && (p.partial ? (p.N & 3) == 0 : p.out.vec != 0);
+            const int row0 = m * kTileM + quarter * 32;
 #pragma unroll 1
-            for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-                const int col = n * BN + c + sub * 4;
-                uint2 rw[8];
-                float b[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int c = c0; c < c1; c += 32) {
+                const int col = n * BN + c;
                 uint32_t v[32];
                 tmem_load32(tmem + (uint32_t)(acc * BN + c) + ((uint32_t)quarter << 21), v);
-                if (whole && !p.partial) {  // on their way while the accumulator is read
-                    if (p.out.residual) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            rw[i] = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(p.out.residual) + (long long)(row0 + i * 4) * p.out.ldr + col));
-                    }
-                    if (p.out.bias) load4(reinterpret_cast<const T*>(p.out.bias) + col, false, 4, b);
-                }
                 tmem_wait_load();
-                if (c + 32 >= (half + 1) * (BN / 2)) {  // the accumulator's last piece is in registers
+                if (c + 32 >= c1) {  // the accumulator's last piece is in registers
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(acc_empty(acc));
                 }
+                if constexpr (kJoins) {
+                    if (p.cluster > 1) {  // for the blocks that join the tile; the ring has done its work
+                        const uint32_t slot = base + (uint32_t)(quarter * (BN / 32) + c / 32) * kPieceBytes;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece + lane * 128 + ((i ^ (lane & 7)) * 16)),
-                                 "r"(v[4 * i]), "r"(v[4 * i + 1]), "r"(v[4 * i + 2]), "r"(v[4 * i + 3])
-                                 : "memory");
-                __syncwarp();
-                if (whole) {
-                    float z[8][4];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int in = i * 4 + (lane >> 3);
-                        uint32_t w[4];
-                        lds128(piece + in * 128 + ((sub ^ (in & 7)) * 16), w[0], w[1], w[2], w[3]);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) z[i][j] = __uint_as_float(w[j]) + b[j];
+                        for (int u = 0; u < 8; ++u) sts128(slot + unit128(lane, u), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+                        fence_async();
+                        continue;
                     }
-                    if (p.partial) {
+                }
+                const auto next = [&] {
+                    if (c + 32 < c1) fetch_residual(p, w, row0, col + 32, lane);
+                    else if (more) fetch_residual(p, w, m2 * kTileM + quarter * 32, n2 * BN + c0, lane);
+                };
+                if (row0 < p.M && col < p.N) {
+                    float z[32];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            *reinterpret_cast<float4*>(p.partial + ((long long)split * p.M + row0 + i * 4) * p.N + col) =
-                                make_float4(z[i][0], z[i][1], z[i][2], z[i][3]);
-                    } else {
-                        const auto residual = [&] {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                z[i][0] += Word<T>::get(rw[i].x, 0);
-                                z[i][1] += Word<T>::get(rw[i].x, 1);
-                                z[i][2] += Word<T>::get(rw[i].y, 0);
-                                z[i][3] += Word<T>::get(rw[i].y, 1);
-                            }
-                        };
-                        const auto store = [&](void* to) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                *reinterpret_cast<uint2*>(reinterpret_cast<T*>(to) + (long long)(row0 + i * 4) * p.out.ldy + col) =
-                                    make_uint2(Word<T>::put(z[i][0], z[i][1]), Word<T>::put(z[i][2], z[i][3]));
-                        };
-                        if (p.out.residual && !p.out.after) residual();
-                        if (p.out.aux) store(p.out.aux);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) z[i][j] = act_value<ACT>(z[i][j]);
-                        if (p.out.residual && p.out.after) residual();
-                        store(p.out.y);
-                    }
-                } else {
-                    const int left = p.N - col;
-                    if (!p.partial && p.out.bias && left > 0) load4(reinterpret_cast<const T*>(p.out.bias) + col, false, left, b);
-#pragma unroll 1
-                    for (int i = 0; i < 8; ++i) {
-                        const int in = i * 4 + (lane >> 3);
-                        const long long row = row0 + i * 4;
-                        uint32_t w[4];
-                        lds128(piece + in * 128 + ((sub ^ (in & 7)) * 16), w[0], w[1], w[2], w[3]);
-                        if (row >= p.M || left <= 0) continue;
-                        float z[4] = {__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]), __uint_as_float(w[3])};
-                        if (p.partial) {
-                            float* to = p.partial + ((long long)split * p.M + row) * p.N + col;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (j < left) to[j] = z[j];
-                        } else {
-                            float r[4] = {0.f, 0.f, 0.f, 0.f};
-                            if (p.out.residual) load4(reinterpret_cast<const T*>(p.out.residual) + row * p.out.ldr + col, p.out.vec, left, r);
-                            finish4<T, ACT>(p.out, row, col, left, z, b, r);
-                        }
+                    for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(v[i]);
+                    finish_piece<T, ACT>(p, w, z, row0, col, split, lane, next);
+                } else if (residual) {  // nothing to finish, but its copy is on the way
+                    if (!w.late && !mbar_wait_for(w.bar, w.phase, p.limit)) w.late = true;
+                    w.phase ^= 1u;
+                    next();
+                }
+            }
+            if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+            m = m2; n = n2; split = split2;
+        }
+        late |= w.late;
+    }
+    if constexpr (kJoins) {
+        if (p.cluster > 1) {
+            // Piece j of the tile is joined by warp j / cluster of block j % cluster.  Every block sends it its own sums.
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();  // no ring of the cluster is in use
+            if (warp >= 4) {
+                int m, n, rank;
+                tile_of(p, blockIdx.x, m, n, rank);
+                const int wj = warp - 4, quarter = warp & 3, half = wj >> 2;
+                const uint32_t received = base + kSlots * kPieceBytes;
+                const auto valid = [&](int j) { return m * kTileM + j / (BN / 32) * 32 < p.M && n * BN + j % (BN / 32) * 32 < p.N; };
+                const int mine = rank + p.cluster * wj;
+                const bool join = mine < kSlots && valid(mine);
+                if (lane == 0) {
+                    if (join) mbar_arrive_expect_tx(join_bar(wj), (uint32_t)p.cluster * kPieceBytes);
+                    for (int c = 0; c < BN / 64; ++c) {
+                        const int j = quarter * (BN / 32) + half * (BN / 64) + c, to = j % p.cluster, at = j / p.cluster;
+                        if (valid(j))
+                            bulk_s2cluster(cluster_map(received + (uint32_t)(at * p.cluster + rank) * kPieceBytes, to), base + (uint32_t)j * kPieceBytes,
+                                           kPieceBytes, cluster_map(join_bar(at), to));
                     }
                 }
                 __syncwarp();
+                if (join) {
+                    const int row0 = m * kTileM + mine / (BN / 32) * 32, col = n * BN + mine % (BN / 32) * 32;
+                    Piece w{pieces + (uint32_t)wj * kPieceBytes, res_bar(wj), 0u, false};
+                    if (p.out.residual && p.boxes) fetch_residual(p, w, row0, col, lane);
+                    if (!mbar_wait_for(join_bar(wj), 0, p.limit)) late = true;
+                    float z[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) z[i] = 0.f;
+                    for (int s = 0; s < p.cluster; ++s) {
+                        const uint32_t from = received + (uint32_t)(wj * p.cluster + s) * kPieceBytes;
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            uint32_t f[4];
+                            lds128(from + unit128(lane, u), f[0], f[1], f[2], f[3]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) z[4 * u + i] += __uint_as_float(f[i]);
+                        }
+                    }
+                    finish_piece<T, ACT>(p, w, z, row0, col, 0, lane, [] {});
+                    late |= w.late;
+                }
             }
-            if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();  // what this block has sent has arrived
         }
     }
+    if (warp >= 4 && lane == 0) tma_store_wait_read();
     if (late) {
         atomicCAS(p.fault, 0, kFaultLinear);
         // what is in flight (copies, products) ends in microseconds
