@@ -94,12 +94,29 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// One lane of a whole warp, always the same.  (Not "lane 0": the copies and products below take their operands from the
+// warp's uniform registers, and only a branch that the compiler knows to be taken by one lane keeps them there.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 // Shared-memory descriptor, 128-byte swizzle (1024-byte aligned tiles of 128-byte rows).
 //   reduction axis innermost: rows of 64 elements, 8 rows are 1024 bytes (stride offset); the leading offset is not used
 //   other axis innermost: 64 elements of it a row, one row for each step of the reduction; 8 rows are 1024 bytes
 //   (stride offset), the next 64 elements lie `leading` bytes on
-__device__ __forceinline__ uint64_t smem_descriptor(uint32_t addr, uint32_t leading) {
-    return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+// The upper half is the same for all; the lower holds the address, so that `lower + bytes / 16` is a descriptor further on.
+__device__ __forceinline__ uint32_t smem_descriptor_lower(uint32_t addr, uint32_t leading) { return (addr & 0x3ffffu) >> 4 | (leading >> 4) << 16; }
+__device__ __forceinline__ uint64_t smem_descriptor(uint32_t lower) {
+    constexpr uint32_t upper = (1024 >> 4) | 1u << 14 | 2u << 29;
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lower), "r"(upper));
+    return d;
 }
 
 }  // namespace ddf
