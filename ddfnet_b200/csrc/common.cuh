@@ -199,6 +199,15 @@ __device__ __forceinline__ void sts16(uint32_t a, uint32_t v) {
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"((uint16_t)v) : "memory");
 }
 
+// 16 bytes that are read once: past the first-level cache.
+__device__ __forceinline__ uint4 ld_granule(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
 // Copy-issuer helper: bytes [g0, g1) of a tensor (16-byte aligned base, `total` bytes) go to
 // shared memory such that byte g lands at dst + (g - (g0 & ~15)).  The aligned superset is
 // fetched by one bulk copy, clamped to the tensor's last whole 16 bytes; what is left of a
@@ -230,6 +239,11 @@ __device__ __forceinline__ void pin(uint32_t& v) { asm volatile("" : "+r"(v)); }
 __device__ __forceinline__ void pin(int& v) { asm volatile("" : "+r"(v)); }
 __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+f"(v)); }
 __device__ __forceinline__ void pin(unsigned long long& v) { asm volatile("" : "+l"(v)); }
+
+// Launches with the programmatic-serialization attribute: the next kernel of the stream may be set up once all blocks of
+// this one have said so; it waits for this one's end, and for its writes, before it touches them.
+__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ------------------------------------------------------------------ packed f32x2
 __device__ __forceinline__ unsigned long long f2_pack(float a, float b) {

@@ -96,56 +96,105 @@ __global__ void __launch_bounds__(32 * kRowsWarps) linear_rows_kernel(const T* _
 }
 
 // ------------------------------------------------------------------ operands that TMA cannot address
-// Rows that do not start on 16 bytes: copied to rows that do.
-template <typename T> __global__ void __launch_bounds__(256) linear_pack_kernel(const T* __restrict__ src, long long ld, T* __restrict__ dst, long long ldp, long long rows, int cols) {
-    for (long long row = blockIdx.y * 8 + (threadIdx.x >> 5); row < rows; row += (long long)gridDim.y * 8)
-#pragma unroll 4
-        for (int c = blockIdx.x * 128 + (threadIdx.x & 31), i = 0; i < 4; ++i, c += 32)
-            if (c < cols) dst[row * ldp + c] = __ldg(src + row * ld + c);
+// Rows that do not start on 16 bytes: copied to rows that do, up to two matrices in a launch.
+struct PackPlan {
+    const void* src[2];
+    void* dst[2];
+    long long ld[2], rows[2];
+    int cols;
+};
+template <typename T> __global__ void __launch_bounds__(256) linear_pack_kernel(const PackPlan p) {
+    const int which = blockIdx.z;
+    const T* src = reinterpret_cast<const T*>(p.src[which]);
+    T* dst = reinterpret_cast<T*>(p.dst[which]);
+    const long long ldp = (p.cols + 7) / 8 * 8;
+    for (long long row = blockIdx.y * 8 + (threadIdx.x >> 5); row < p.rows[which]; row += (long long)gridDim.y * 8) {
+        const T* from = src + row * p.ld[which];
+        const int c = blockIdx.x * 256 + (threadIdx.x & 31);
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i * 32 < p.cols) v[i] = __ldg(from + c + i * 32);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i * 32 < p.cols) dst[row * ldp + c + i * 32] = v[i];
+    }
 }
 
 // ------------------------------------------------------------------ backward of what follows the product
 // gz = gy act'(.) into up to two buffers, and its sums over `chunk` rows of each column.  Bound by bytes: gy and
-// aux read once, gz written once.  A warp takes 128 columns of a row at a time.
+// aux read once, gz written once.  A warp takes 256 columns of a row at a time, eight a lane, four rows in flight.
 struct BackPlan {
     const void *gy, *aux;
     void *gz, *gz2;    // either may be NULL; rows ldz / N apart
     float* sums;       // chunks x N, or NULL
     long long ldg, ldz, M;
-    int N, chunk, vec, vecz;
+    int N, chunk;
 };
-template <typename T, int ACT> __global__ void __launch_bounds__(256) linear_back_kernel(const BackPlan p) {
-    __shared__ float4 sums[8][32];
+// Eight elements of a row, the first `n` of them, as they lie in memory.
+template <typename T, bool VEC> __device__ __forceinline__ uint4 load8(const T* p, int n) {
+    if constexpr (VEC) return ld_granule(p);  // (N is a multiple of eight)
+    uint32_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        q[i] = Word<T>::put(2 * i < n ? Elem<T>::load(p + 2 * i) : 0.f, 2 * i + 1 < n ? Elem<T>::load(p + 2 * i + 1) : 0.f);
+    return make_uint4(q[0], q[1], q[2], q[3]);
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, bool vec, int n, const uint4& v) {
+    if (vec && n >= 8) {
+        *reinterpret_cast<uint4*>(p) = v;
+    } else {
+        const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) Elem<T>::store(p + i, Word<T>::get(q[i / 2], i % 2));
+    }
+}
+template <typename T, int ACT, bool VEC> __global__ void __launch_bounds__(256) linear_back_kernel(const BackPlan p) {
+    __shared__ float sums[8][256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int col = blockIdx.x * 128 + lane * 4, left = p.N - col;
+    const int col = blockIdx.x * 256 + lane * 8, left = p.N - col;
     const long long r0 = (long long)blockIdx.y * p.chunk, r1 = min(p.M, r0 + p.chunk);
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    float s[8] = {};
     if (left > 0) {
-#pragma unroll 4
-        for (long long r = r0 + warp; r < r1; r += 8) {
-            float g[4], z[4];
-            load4(reinterpret_cast<const T*>(p.gy) + r * p.ldg + col, p.vec, left, g);
-            if constexpr (ACT != kActNone) {
-                load4(reinterpret_cast<const T*>(p.aux) + r * p.N + col, p.vec, left, z);
+        constexpr int FLIGHT = 4;
+        for (long long r = r0 + warp; r < r1; r += 8 * FLIGHT) {
+            uint4 g[FLIGHT], z[FLIGHT];  // (rows past the end: the last one again)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) g[i] *= act_slope<ACT>(z[i]);
+            for (int f = 0; f < FLIGHT; ++f) {
+                const long long row = min(r + 8 * f, r1 - 1);
+                g[f] = load8<T, VEC>(reinterpret_cast<const T*>(p.gy) + row * p.ldg + col, left);
+                if constexpr (ACT != kActNone) z[f] = load8<T, VEC>(reinterpret_cast<const T*>(p.aux) + row * p.N + col, left);
             }
-            if (p.gz) store4(reinterpret_cast<T*>(p.gz) + r * p.ldz + col, p.vecz, left, g);
-            if (p.gz2) store4(reinterpret_cast<T*>(p.gz2) + r * p.N + col, p.vec, left, g);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] += g[i];
+            for (int f = 0; f < FLIGHT; ++f) {
+                if (r + 8 * f >= r1) break;
+                const uint32_t a[4] = {g[f].x, g[f].y, g[f].z, g[f].w};
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = Word<T>::get(a[i / 2], i % 2);
+                if constexpr (ACT != kActNone) {
+                    const uint32_t b[4] = {z[f].x, z[f].y, z[f].z, z[f].w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] *= act_slope<ACT>(Word<T>::get(b[i / 2], i % 2));
+                    g[f] = make_uint4(Word<T>::put(v[0], v[1]), Word<T>::put(v[2], v[3]), Word<T>::put(v[4], v[5]), Word<T>::put(v[6], v[7]));
+                }
+                if (p.gz) store8(reinterpret_cast<T*>(p.gz) + (r + 8 * f) * p.ldz + col, true, left, g[f]);  // (the workspace's rows)
+                if (p.gz2) store8(reinterpret_cast<T*>(p.gz2) + (r + 8 * f) * p.N + col, VEC, left, g[f]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i] += v[i];
+            }
         }
     }
     if (!p.sums) return;
-    sums[warp][lane] = make_float4(s[0], s[1], s[2], s[3]);
-    __syncthreads();
-    if (threadIdx.x < 128) {
-        const int c = blockIdx.x * 128 + threadIdx.x;
-        float all = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) all += reinterpret_cast<const float*>(&sums[w][0])[threadIdx.x];
-        if (c < p.N) p.sums[(long long)blockIdx.y * p.N + c] = all;
-    }
+    for (int i = 0; i < 8; ++i) sums[warp][lane * 8 + i] = s[i];
+    __syncthreads();
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) all += sums[w][threadIdx.x];
+    if (c < p.N) p.sums[(long long)blockIdx.y * p.N + c] = all;
 }
 // Column sums of the chunks' sums, in one order.
 template <typename T> __global__ void __launch_bounds__(256) linear_bias_kernel(const float* __restrict__ sums, T* __restrict__ gb, int chunks, int N) {
@@ -153,7 +202,7 @@ template <typename T> __global__ void __launch_bounds__(256) linear_bias_kernel(
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float s = 0.f;
     if (c < N)
-#pragma unroll 4
+#pragma unroll 8
         for (int i = warp; i < chunks; i += 8) s += __ldg(sums + (long long)i * N + c);
     part[warp][lane] = s;
     __syncthreads();
@@ -206,36 +255,36 @@ static int encode_matrix(CUtensorMap* map, const Matrix& m, int dtype, int box_c
                   box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// How a product is cut: columns of a tile, splits of K, and whether a cluster of blocks joins them.
+// How a product is cut: columns of a tile and splits of K.  By an estimate of the time, from measurements on products of
+// 8 to 8192 rows (clocks of a step of 64 along K, of an epilogue that nothing hides, microseconds of a launch's start and
+// end, and of the join).  32x4096x4096: 128 columns, 4 splits 10.8 us, no split 16.9, 64 columns 15.3.  256x2048x1000: 64
+// columns, 3 splits 8.6, no split 9.7, 256 columns 14.1.  2048x2048x2048: 256 columns 15.7, 128 19.2, with 2 splits 25.5.
 struct Cut {
     int bn, splits, steps;
-    bool cluster;
 };
 static Cut cut_of(long long M, long long N, long long K, int sm_count) {
     const long long steps = (K + kTileK - 1) / kTileK, tiles_m = (M + kTileM - 1) / kTileM;
-    Cut best{256, 1, (int)steps, false};
+    Cut best{256, 1, (int)steps};
     double least = 1e300;
     for (int bn : {256, 128, 64}) {
         if (bn > 64 && N <= bn / 2) continue;
-        // clocks of a step of 64 along K, and of a tile's start and end
-        const double step = bn == 256 ? 600 : bn == 128 ? 370 : 260, once = 1200 + 5 * bn;
+        const double step = bn == 256 ? 530 : bn == 128 ? 380 : 340, epilogue = 1300 + 20 * bn;
         const long long tiles = tiles_m * ((N + bn - 1) / bn);
-        for (int want : {1, 2, 4, 8, 12, 16, 24, 32, 48}) {
+        for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48}) {
             const long long per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
-            if (splits > 1 && (per < 2 || (splits > 8 && (double)splits * M * N > 64e6))) break;
-            const bool cluster = splits > 1 && splits <= 8 && bn <= 128;
+            if (splits > 1 && (per < 2 || (double)splits * M * N > 64e6)) break;
             const long long waves = (tiles * splits + sm_count - 1) / sm_count;
-            const double join = cluster ? 1500 : splits > 1 ? 4000 + (double)M * N * (8 * splits + 4) / 3000 : 0;
-            const double cost = (double)waves * (per * step + once + (cluster ? join : 0)) + (cluster ? 0 : join);
-            if (cost < least * 0.97) {
-                least = cost;
-                best = Cut{bn, (int)splits, (int)per, cluster};
+            const double busy = per * step > epilogue ? per * step : epilogue;
+            const double us = 4.0 + 0.0045 * bn + (per * step + (waves - 1) * busy) / 1900 + (splits > 1 ? 1.2 + (double)M * N * splits * 8 / 4.2e6 : 0);
+            if (us < least) {
+                least = us;
+                best = Cut{bn, (int)splits, (int)per};
             }
         }
     }
     return best;
 }
-static size_t partial_bytes(long long M, long long N, const Cut& c) { return c.splits > 1 && !c.cluster ? (size_t)c.splits * M * N * 4 : 0; }
+static size_t partial_bytes(long long M, long long N, const Cut& c) { return c.splits > 1 ? (size_t)c.splits * M * N * 4 : 0; }
 
 template <typename T, bool AT, bool BT> static auto kernel_of(int bn, int act) {
     if constexpr (!AT && !BT) {
@@ -254,10 +303,10 @@ static int product(const Matrix& a, const Matrix& b, long long M, long long N, l
     int rc = device_facts(&sm, &fault, &index);
     if (rc) return rc;
     const Cut cut = cut_of(M, N, K, sm);
-    const bool joined = cut.splits > 1 && !cut.cluster;  // by a kernel of its own, which finishes too
+    const bool joined = cut.splits > 1;  // by a kernel of its own, which finishes too
     auto kernel = kernel_of<T, AT, BT>(cut.bn, joined ? (int)kActNone : out.act);
     // (before the driver's encoder: a runtime call gives a thread that has none its context)
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinearShared);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)linear_shared(cut.bn));
     if (e != cudaSuccess) return (int)e;
     LinearPlan p{};
     if ((rc = encode_matrix(&p.a, a, dtype, 64, AT ? kTileK : kTileM))) return rc;
@@ -283,7 +332,6 @@ static int product(const Matrix& a, const Matrix& b, long long M, long long N, l
     p.tiles_n = (int)((N + cut.bn - 1) / cut.bn);
     p.splits = cut.splits;
     p.steps = cut.steps;
-    p.cluster = cut.cluster ? cut.splits : 1;
     const uint32_t type = dtype == DDF_B200_BF16 ? 1u : 0u;
     p.idesc = 1u << 4 | type << 7 | type << 10 | (AT ? 1u << 15 : 0u) | (BT ? 1u << 16 : 0u) | (uint32_t)(cut.bn / 8) << 17 | (uint32_t)(kTileM / 16) << 24;
     p.fault = fault;
@@ -291,22 +339,24 @@ static int product(const Matrix& a, const Matrix& b, long long M, long long N, l
     const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
     if (items > 0x7fffffffll) return DDF_B200_E_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(cut.cluster || items < sm ? items : sm));
+    cfg.gridDim = dim3((unsigned)(items < sm ? items : sm));
     cfg.blockDim = dim3(kLinearThreads);
-    cfg.dynamicSmemBytes = kLinearShared;
+    cfg.dynamicSmemBytes = linear_shared(cut.bn);
     cfg.stream = st;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)p.cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = cut.cluster ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e != cudaSuccess) return (int)e;
     rc = launched();
     if (rc || !joined) return rc;
-    linear_join_kernel<T><<<(unsigned)((M * ((N + 3) / 4) + 255) / 256), 256, 0, st>>>(partial, out, (int)M, (int)N, cut.splits);
-    return launched();
+    cfg.gridDim = dim3((unsigned)((M * ((N + 3) / 4) + 63) / 64));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    cudaLaunchAttribute attr = {};  // set up while the product runs
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, linear_join_kernel<T>, (const float*)partial, out, (int)M, (int)N, cut.splits);
+    return e != cudaSuccess ? (int)e : launched();
 }
 
 constexpr int kFewRows = 4;
@@ -322,10 +372,33 @@ template <typename T, int MR, int CW> static int rows_launch(const ddf_b200_line
     return launched();
 }
 
-template <typename T> static int pack(const Matrix& m, void* to, cudaStream_t st) {
-    const long long tall = (m.rows + 7) / 8;
-    linear_pack_kernel<T><<<dim3((unsigned)((m.cols + 127) / 128), (unsigned)(tall < 32768 ? tall : 32768)), 256, 0, st>>>((const T*)m.p, m.ld, (T*)to, padded(m.cols), m.rows, (int)m.cols);
+// Copies x and w, where `xp` / `wp` is a place for them, and has them point there.
+template <typename T> static int pack(Matrix& x, void* xp, Matrix& w, void* wp, cudaStream_t st) {
+    PackPlan p{};
+    int n = 0;
+    long long tall = 0;
+    Matrix* const both[2] = {&x, &w};
+    void* const to[2] = {xp, wp};
+    for (int i = 0; i < 2; ++i) {
+        if (!to[i]) continue;
+        Matrix& m = *both[i];
+        p.src[n] = m.p; p.dst[n] = to[i]; p.ld[n] = m.ld; p.rows[n] = m.rows;
+        p.cols = (int)m.cols;
+        tall = m.rows > tall ? m.rows : tall;
+        m.p = to[i]; m.ld = padded(m.cols);
+        ++n;
+    }
+    if (!n) return 0;
+    tall = (tall + 7) / 8;
+    linear_pack_kernel<T><<<dim3((unsigned)((p.cols + 255) / 256), (unsigned)(tall < 4096 ? tall : 4096), (unsigned)n), 256, 0, st>>>(p);
     return launched();
+}
+
+template <typename T> static auto back_kernel_of(int act, bool vec) {
+    if (act == kActRelu) return vec ? linear_back_kernel<T, kActRelu, true> : linear_back_kernel<T, kActRelu, false>;
+    if (act == kActGelu) return vec ? linear_back_kernel<T, kActGelu, true> : linear_back_kernel<T, kActGelu, false>;
+    if (act == kActSilu) return vec ? linear_back_kernel<T, kActSilu, true> : linear_back_kernel<T, kActSilu, false>;
+    return vec ? linear_back_kernel<T, kActNone, true> : linear_back_kernel<T, kActNone, false>;
 }
 
 // Workspace: consecutive blocks, 256-byte aligned.
@@ -363,20 +436,12 @@ static int forward(const ddf_b200_linear_args* q, void* y, void* aux, Space& ws,
     }
     Matrix x{q->x, M, K, q->x_stride}, w{q->weight, N, K, q->weight_stride};
     void* xp = addressable(x.p, x.ld) ? nullptr : ws.take((size_t)M * padded(K) * 2);
-    const bool pack_x = !addressable(x.p, x.ld), pack_w = !addressable(w.p, w.ld);
-    void* wp = pack_w ? ws.take((size_t)N * padded(K) * 2) : nullptr;
+    void* wp = addressable(w.p, w.ld) ? nullptr : ws.take((size_t)N * padded(K) * 2);
     float* partial = (float*)ws.take(partial_bytes(M, N, cut_of(M, N, K, sm)));
     if (only_size) return 0;
     if (ws.used > have) return DDF_B200_E_WORKSPACE;
-    int rc;
-    if (pack_x) {
-        if ((rc = pack<T>(x, xp, st))) return rc;
-        x.p = xp; x.ld = padded(K);
-    }
-    if (pack_w) {
-        if ((rc = pack<T>(w, wp, st))) return rc;
-        w.p = wp; w.ld = padded(K);
-    }
+    const int rc = pack<T>(x, xp, w, wp, st);
+    if (rc) return rc;
     return product<T, false, false>(x, w, M, N, K, e, partial, q->dtype, limit, st);
 }
 
@@ -393,9 +458,10 @@ static int backward(const ddf_b200_linear_args* q, const void* gy, long long gy_
     Matrix gz{as_gy ? gy : as_gr ? gr : nullptr, M, N, as_gy ? gy_stride : as_gr ? N : padded(N)};
     void* gzp = scratch ? ws.take((size_t)M * padded(N) * 2) : nullptr;
     if (scratch) gz.p = gzp;
-    const long long most = 256;  // chunks of rows for the column sums
-    long long chunk = (M + most - 1) / most;
-    chunk = chunk < 64 ? 64 : (chunk + 7) / 8 * 8;
+    // rows of a block: four blocks an SM, 512 sums a column at most
+    long long chunk = M * ((N + 255) / 256) / (4 * sm);
+    chunk = chunk < (M + 511) / 512 ? (M + 511) / 512 : chunk;
+    chunk = (chunk + 8) / 8 * 8;
     const long long chunks = (M + chunk - 1) / chunk;
     float* sums = gb ? (float*)ws.take((size_t)chunks * N * 4) : nullptr;
     Matrix x{q->x, M, K, q->x_stride}, w{q->weight, N, K, q->weight_stride};
@@ -414,26 +480,17 @@ static int backward(const ddf_b200_linear_args* q, const void* gy, long long gy_
 
     int rc;
     if (scratch || want_gr || gb) {
-        BackPlan b{gy, aux, scratch ? gzp : nullptr, want_gr ? gr : nullptr, sums, gy_stride, padded(N), M, (int)N, (int)chunk, 0, 0};
-        b.vec = by_four(gy, gy_stride) && (!act || by_four(aux, N)) && (!want_gr || by_four(gr, N));
-        b.vecz = 1;
-        auto kernel = q->activation == kActRelu ? linear_back_kernel<T, kActRelu> : q->activation == kActGelu ? linear_back_kernel<T, kActGelu>
-                      : q->activation == kActSilu ? linear_back_kernel<T, kActSilu> : linear_back_kernel<T, kActNone>;
-        kernel<<<dim3((unsigned)((N + 127) / 128), (unsigned)chunks), 256, 0, st>>>(b);
+        const BackPlan b{gy, aux, scratch ? gzp : nullptr, want_gr ? gr : nullptr, sums, gy_stride, padded(N), M, (int)N, (int)chunk};
+        const bool vec = N % 8 == 0 && addressable(gy, gy_stride) && (!act || addressable(aux, N)) && (!want_gr || addressable(gr, N));
+        auto kernel = back_kernel_of<T>(q->activation, vec);
+        kernel<<<dim3((unsigned)((N + 255) / 256), (unsigned)chunks), 256, 0, st>>>(b);
         if ((rc = launched())) return rc;
         if (gb) {
             linear_bias_kernel<T><<<(unsigned)((N + 31) / 32), 256, 0, st>>>(sums, (T*)gb, (int)chunks, (int)N);
             if ((rc = launched())) return rc;
         }
     }
-    if (pack_x) {
-        if ((rc = pack<T>(x, xp, st))) return rc;
-        x.p = xp; x.ld = padded(K);
-    }
-    if (pack_w) {
-        if ((rc = pack<T>(w, wp, st))) return rc;
-        w.p = wp; w.ld = padded(K);
-    }
+    if ((rc = pack<T>(x, xp, w, wp, st))) return rc;
     Epilogue e{};
     if (gx) {
         e.y = gx; e.ldy = K; e.vec = by_four(gx, K);

@@ -9,14 +9,15 @@
 //
 // What bounds it: 2 M N K operations at the tensor cores' rate, or, with few rows or small K, the operands' and
 // results' bytes.  One persistent block an SM:
-//   warp 0     one thread loads tiles of 64 along K by TMA into a ring of stages (192 KB)
+//   warp 0     one thread loads tiles of 64 along K by TMA into a ring of stages
 //   warp 1     one thread issues the products, 128 x BN, into one of two accumulators in tensor memory
 //   warps 4-11 take the other accumulator meanwhile, in pieces of 32 x 32: a thread holds a row of it; residual and
 //              results pass through shared memory to and from TMA, whose copies the warp does not wait for
 // BN = 256 where the tiles fill the machine: a 128 x 256 tile's operands take 96 bytes of shared memory a clock
-// at the full rate, a 128 x 128 tile's all 128.  Where they would not, smaller BN and splits of K: up to eight
-// blocks of a cluster take one tile, and join its pieces out of each other's shared memory, in the order of K; more
-// splits leave partial sums in the workspace, joined in that order by linear_join_kernel.
+// at the full rate, a 128 x 128 tile's all 128.  Where they would not, smaller BN and splits of K, whose partial sums
+// linear_join_kernel joins in the order of K; it is set up while this kernel runs.  (A cluster of blocks that joined
+// them out of each other's shared memory gained at most half a microsecond where all its blocks fit at once, and lost
+// eight where they did not.)
 //
 // Every wait is bounded: a role whose wait runs out records a fault and leaves its loop, the others follow by their
 // own limits; the block meets after a pause in which its copies land, frees the tensor memory and ends.
@@ -29,9 +30,16 @@ namespace ddf {
 constexpr int kFaultLinear = 6;  // a wait of linear_kernel ran out
 constexpr int kTileM = 128, kTileK = 64;
 constexpr int kLinearThreads = 384, kJoinWarps = 8;
-constexpr uint32_t kRingBytes = 192 * 1024;
-constexpr uint32_t kPieceBytes = 32 * 32 * 4;  // an epilogue warp's piece
-constexpr uint32_t kLinearShared = kRingBytes + kJoinWarps * kPieceBytes + 1024 + 512;
+// Shared memory: the ring of stages, and for every epilogue warp boxes of 2 KB (32 x 32 of a 2-byte type).  Wide tiles take
+// four stages and two boxes; narrower ones, which small K is for, five or six stages and four boxes: results
+// leave from two of them in turn, residuals arrive in the others.
+constexpr uint32_t kBox = 2048;
+__host__ __device__ constexpr uint32_t stage_bytes(int bn) { return (uint32_t)(kTileM + bn) * kTileK * 2; }
+__host__ __device__ constexpr int stages_of(int bn) { return bn == 256 ? 4 : bn == 128 ? 5 : 6; }
+__host__ __device__ constexpr int boxes_of(int bn) { return bn == 256 ? 2 : 4; }
+__host__ __device__ constexpr uint32_t linear_shared(int bn) {
+    return stages_of(bn) * stage_bytes(bn) + kJoinWarps * boxes_of(bn) * kBox + 1024 + 512;
+}
 
 enum Act { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
 
@@ -117,7 +125,7 @@ template <typename T> __device__ __forceinline__ void store4(T* p, bool vec, int
 }
 
 // bias, residual, activation and the stores of four elements of a row: `b` and `r` are 0 where there is none.
-template <typename T, int ACT = -1>  // -1: as e.act says
+template <typename T>
 __device__ __forceinline__ void finish4(const Epilogue& e, long long row, int col, int n, float (&z)[4], const float (&b)[4], const float (&r)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -126,10 +134,7 @@ __device__ __forceinline__ void finish4(const Epilogue& e, long long row, int co
     }
     if (e.aux) store4(reinterpret_cast<T*>(e.aux) + row * e.ldy + col, e.vec, n, z);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (ACT < 0) z[i] = act_value(z[i], e.act);
-        else z[i] = act_value<ACT>(z[i]);
-    }
+    for (int i = 0; i < 4; ++i) z[i] = act_value(z[i], e.act);
     if (e.after) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) z[i] += r[i];
@@ -144,7 +149,6 @@ struct LinearPlan {
     float* partial;         // splits x M x N, where the workspace joins them
     int M, N, K;
     int tiles_m, tiles_n, splits, steps;  // steps of 64 along K in a split
-    int cluster;            // blocks that share a tile, each with its split
     int boxes;              // TMA can address the outputs and the residual
     int bias_vec;           // ... and 16-byte loads the bias
     uint32_t idesc;
@@ -155,14 +159,8 @@ struct LinearPlan {
 // Work item -> tile and split: tiles of eight blocks of rows side by side, so that the tiles in flight share operands.
 __device__ __forceinline__ void tile_of(const LinearPlan& p, int item, int& m, int& n, int& split) {
     const int tiles = p.tiles_m * p.tiles_n;
-    int t;
-    if (p.cluster > 1) {
-        t = item / p.cluster;
-        split = item - t * p.cluster;
-    } else {
-        split = item / tiles;
-        t = item - split * tiles;
-    }
+    split = item / tiles;
+    const int t = item - split * tiles;
     const int group = t / (8 * p.tiles_n), in = t - group * 8 * p.tiles_n;
     const int rows = min(8, p.tiles_m - group * 8);
     m = group * 8 + in % rows;
@@ -171,29 +169,46 @@ __device__ __forceinline__ void tile_of(const LinearPlan& p, int item, int& m, i
 
 // What an epilogue warp needs to finish a piece of 32 rows x 32 columns, one row a lane.
 struct Piece {
-    uint32_t stage;   // 4 KB: results, then (from 2 KB on) the residual; or floats
-    uint32_t bar;     // of the residual's copy
-    uint32_t phase;
+    uint32_t stage;      // its boxes: `outs` for results, then `ins` for residuals
+    uint32_t bar;        // of the first residual box's copy; the second's follows
+    int outs, ins;
+    int out, in;         // the next of each
+    uint32_t phases;     // of the residual boxes' barriers, a bit each
     bool late;
 };
 // 16-byte unit u of row `lane` of a box of 64-byte rows (64-byte swizzle) or 128-byte rows (128-byte swizzle).
 __device__ __forceinline__ uint32_t unit64(int lane, int u) { return lane * 64 + ((u ^ (lane >> 1 & 3)) * 16); }
 __device__ __forceinline__ uint32_t unit128(int lane, int u) { return lane * 128 + ((u ^ (lane & 7)) * 16); }
 
-__device__ __forceinline__ void fetch_residual(const LinearPlan& p, const Piece& w, int row0, int col, int lane) {
+__device__ __forceinline__ void fetch_residual(const LinearPlan& p, const Piece& w, int box, int row0, int col, int lane) {
     if (lane == 0) {
-        mbar_arrive_expect_tx(w.bar, 2048);
-        tma_load_2d(w.stage + 2048, &p.r, col, row0, w.bar);
+        const uint32_t bar = w.bar + 8u * box;
+        mbar_arrive_expect_tx(bar, kBox);
+        tma_load_2d(w.stage + (w.outs + box) * kBox, &p.r, col, row0, bar);
     }
 }
+// Waits for the residual of the next piece; its box's address.
+__device__ __forceinline__ uint32_t await_residual(const LinearPlan& p, Piece& w) {
+    if (!w.late && !mbar_wait_for(w.bar + 8u * w.in, w.phases >> w.in & 1u, p.limit)) w.late = true;
+    w.phases ^= 1u << w.in;
+    return w.stage + (w.outs + w.in) * kBox;
+}
+// Before a box for results is written again.
+__device__ __forceinline__ void await_out(const Piece& w, int lane) {
+    if (lane == 0) {
+        if (w.outs > 1) tma_store_wait_read<1>();
+        else tma_store_wait_read<0>();
+    }
+    __syncwarp();
+}
 
-// `next`: called when the residual of this piece is in registers.  v: the lane's row of the product.
+// z: the lane's row of the product.  `next(box)`: called when the residual in `box` is in registers.
 template <typename T, int ACT, typename Next>
 __device__ __forceinline__ void finish_piece(const LinearPlan& p, Piece& w, float (&z)[32], int row0, int col, int split, int lane, Next next) {
     const Epilogue& e = p.out;
     if (p.partial) {
         if (p.boxes) {
-            if (lane == 0) tma_store_wait_read();
+            if (lane == 0) tma_store_wait_read<0>();
             __syncwarp();
 #pragma unroll
             for (int u = 0; u < 8; ++u)
@@ -225,31 +240,32 @@ __device__ __forceinline__ void finish_piece(const LinearPlan& p, Piece& w, floa
         }
         uint32_t r[16];
         if (e.residual) {
-            if (!w.late && !mbar_wait_for(w.bar, w.phase, p.limit)) w.late = true;
-            w.phase ^= 1u;
+            const uint32_t from = await_residual(p, w);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) lds128v(w.stage + 2048 + unit64(lane, u), r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
+            for (int u = 0; u < 4; ++u) lds128v(from + unit64(lane, u), r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
             fence_async();  // these reads come before the next copy's writes: the warp's barrier alone does not see to that
             __syncwarp();
-            next();
+            next(w.in);
+            if (++w.in == w.ins) w.in = 0;
         }
         const auto add = [&] {
 #pragma unroll
             for (int i = 0; i < 32; ++i) z[i] += Word<T>::get(r[i / 2], i % 2);
         };
         const auto store = [&](const CUtensorMap* map) {
-            if (lane == 0) tma_store_wait_read();
-            __syncwarp();
+            const uint32_t to = w.stage + w.out * kBox;
+            await_out(w, lane);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                sts128(w.stage + unit64(lane, u), Word<T>::put(z[8 * u], z[8 * u + 1]), Word<T>::put(z[8 * u + 2], z[8 * u + 3]),
+                sts128(to + unit64(lane, u), Word<T>::put(z[8 * u], z[8 * u + 1]), Word<T>::put(z[8 * u + 2], z[8 * u + 3]),
                        Word<T>::put(z[8 * u + 4], z[8 * u + 5]), Word<T>::put(z[8 * u + 6], z[8 * u + 7]));
             fence_async();
             __syncwarp();
             if (lane == 0) {
-                tma_store_2d(map, w.stage, col, row0);
+                tma_store_2d(map, to, col, row0);
                 tma_store_commit();
             }
+            if (++w.out == w.outs) w.out = 0;
         };
         if (e.residual && !e.after) add();
         if (e.aux) store(&p.aux);
@@ -289,19 +305,16 @@ __device__ __forceinline__ void finish_piece(const LinearPlan& p, Piece& w, floa
 
 template <typename T, int BN, bool AT, bool BT, int ACT>
 __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_constant__ LinearPlan p) {
-    constexpr uint32_t kA = kTileM * kTileK * 2, kB = BN * kTileK * 2, kStage = kA + kB;
-    constexpr int kStages = (int)(kRingBytes / kStage);
-    constexpr int kSlots = 4 * (BN / 32);  // pieces of a tile
-    constexpr bool kJoins = 2 * kSlots * kPieceBytes <= kRingBytes;  // a tile's sums, sent and received, fit the ring
+    constexpr uint32_t kA = kTileM * kTileK * 2, kStage = stage_bytes(BN);
+    constexpr int kStages = stages_of(BN), kBoxes = boxes_of(BN);
     extern __shared__ unsigned char linear_raw[];
     const uint32_t base = (smem_u32(linear_raw) + 1023u) & ~1023u;
-    const uint32_t pieces = base + kRingBytes, bars = pieces + kJoinWarps * kPieceBytes;
+    const uint32_t pieces = base + kStages * kStage, bars = pieces + kJoinWarps * kBoxes * kBox;
     const auto full = [&](int s) { return bars + 8u * s; };
     const auto empty = [&](int s) { return bars + 8u * (kStages + s); };
     const auto acc_full = [&](int s) { return bars + 8u * (2 * kStages + s); };
     const auto acc_empty = [&](int s) { return bars + 8u * (2 * kStages + 2 + s); };
-    const auto res_bar = [&](int w) { return bars + 8u * (2 * kStages + 4 + w); };
-    const auto join_bar = [&](int w) { return bars + 8u * (2 * kStages + 4 + kJoinWarps + w); };
+    const auto res_bar = [&](int w) { return bars + 8u * (2 * kStages + 4 + 2 * w); };
     const uint32_t tmem_word = bars + 8u * (2 * kStages + 4 + 2 * kJoinWarps);
     const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be the warp's)
     const int items = p.tiles_m * p.tiles_n * p.splits;
@@ -317,12 +330,16 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
             mbar_init(acc_full(s), 1);
             mbar_init(acc_empty(s), kJoinWarps);
         }
-        for (int w = 0; w < 2 * kJoinWarps; ++w) mbar_init(res_bar(w), 1);  // (join_bar too)
+        for (int w = 0; w < kJoinWarps; ++w) {
+            mbar_init(res_bar(w), 1);
+            mbar_init(res_bar(w) + 8u, 1);
+        }
         mbar_fence_init();
         tma_prefetch_map(&p.a);
         tma_prefetch_map(&p.b);
         if (p.boxes) tma_prefetch_map(&p.y);
     }
+    if (p.partial) dependents_may_start();  // the joining kernel; it waits for this one's end before it reads
     if (warp == 2) tmem_alloc(tmem_word, 2 * BN);
     tc_fence_before();
     __syncthreads();
@@ -392,17 +409,28 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
     } else if (warp >= 4) {
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const int c0 = half * (BN / 2), c1 = c0 + BN / 2;
-        Piece w{pieces + (uint32_t)(warp - 4) * kPieceBytes, res_bar(warp - 4), 0u, false};
         const bool residual = p.out.residual && p.boxes && !p.partial;
+        const int ins = residual ? kBoxes / 2 : 0;
+        Piece w{pieces + (uint32_t)(warp - 4) * kBoxes * kBox, res_bar(warp - 4), residual ? kBoxes / 2 : 2, ins, 0, 0, 0u, false};
+        // the residuals' copies run `ins` pieces ahead
+        int fetch_item = blockIdx.x, fetch_c = c0, fetch_m = 0, fetch_n = 0, unused;
+        if (residual && fetch_item < items) tile_of(p, fetch_item, fetch_m, fetch_n, unused);
+        const auto next = [&](int box) {
+            if (fetch_item >= items) return;
+            fetch_residual(p, w, box, fetch_m * kTileM + quarter * 32, fetch_n * BN + fetch_c, lane);
+            fetch_c += 32;
+            if (fetch_c == c1) {
+                fetch_c = c0;
+                fetch_item += gridDim.x;
+                if (fetch_item < items) tile_of(p, fetch_item, fetch_m, fetch_n, unused);
+            }
+        };
+        for (int box = 0; box < ins; ++box) next(box);
         int acc = 0;
         uint32_t acc_phase = 0;
-        int m = 0, n = 0, split = 0;
-        if (blockIdx.x < items) tile_of(p, blockIdx.x, m, n, split);
-        if (residual && p.cluster == 1 && blockIdx.x < items) fetch_residual(p, w, m * kTileM + quarter * 32, n * BN + c0, lane);
         for (int item = blockIdx.x; item < items; item += gridDim.x) {
-            int m2 = 0, n2 = 0, split2 = 0;
-            const bool more = item + (int)gridDim.x < items;
-            if (more) tile_of(p, item + gridDim.x, m2, n2, split2);
+            int m, n, split;
+            tile_of(p, item, m, n, split);
             if (!mbar_wait_for(acc_full(acc), acc_phase, p.limit)) { late = true; break; }
             tc_fence_after();
             const int row0 = m * kTileM + quarter * 32;
@@ -417,87 +445,23 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
                     __syncwarp();
                     if (lane == 0) mbar_arrive(acc_empty(acc));
                 }
-                if constexpr (kJoins) {
-                    if (p.cluster > 1) {  // for the blocks that join the tile; the ring has done its work
-                        const uint32_t slot = base + (uint32_t)(quarter * (BN / 32) + c / 32) * kPieceBytes;
-#pragma unroll
-                        for (int u = 0; u < 8; ++u) sts128(slot + unit128(lane, u), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-                        fence_async();
-                        continue;
-                    }
-                }
-                const auto next = [&] {
-                    if (c + 32 < c1) fetch_residual(p, w, row0, col + 32, lane);
-                    else if (more) fetch_residual(p, w, m2 * kTileM + quarter * 32, n2 * BN + c0, lane);
-                };
                 if (row0 < p.M && col < p.N) {
                     float z[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(v[i]);
                     finish_piece<T, ACT>(p, w, z, row0, col, split, lane, next);
                 } else if (residual) {  // nothing to finish, but its copy is on the way
-                    if (!w.late && !mbar_wait_for(w.bar, w.phase, p.limit)) w.late = true;
-                    w.phase ^= 1u;
-                    next();
+                    await_residual(p, w);
+                    __syncwarp();
+                    next(w.in);
+                    if (++w.in == w.ins) w.in = 0;
                 }
             }
             if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
-            m = m2; n = n2; split = split2;
         }
         late |= w.late;
     }
-    if constexpr (kJoins) {
-        if (p.cluster > 1) {
-            // Piece j of the tile is joined by warp j / cluster of block j % cluster.  Every block sends it its own sums.
-            __syncwarp();
-            cluster_arrive();
-            cluster_wait();  // no ring of the cluster is in use
-            if (warp >= 4) {
-                int m, n, rank;
-                tile_of(p, blockIdx.x, m, n, rank);
-                const int wj = warp - 4, quarter = warp & 3, half = wj >> 2;
-                const uint32_t received = base + kSlots * kPieceBytes;
-                const auto valid = [&](int j) { return m * kTileM + j / (BN / 32) * 32 < p.M && n * BN + j % (BN / 32) * 32 < p.N; };
-                const int mine = rank + p.cluster * wj;
-                const bool join = mine < kSlots && valid(mine);
-                if (lane == 0) {
-                    if (join) mbar_arrive_expect_tx(join_bar(wj), (uint32_t)p.cluster * kPieceBytes);
-                    for (int c = 0; c < BN / 64; ++c) {
-                        const int j = quarter * (BN / 32) + half * (BN / 64) + c, to = j % p.cluster, at = j / p.cluster;
-                        if (valid(j))
-                            bulk_s2cluster(cluster_map(received + (uint32_t)(at * p.cluster + rank) * kPieceBytes, to), base + (uint32_t)j * kPieceBytes,
-                                           kPieceBytes, cluster_map(join_bar(at), to));
-                    }
-                }
-                __syncwarp();
-                if (join) {
-                    const int row0 = m * kTileM + mine / (BN / 32) * 32, col = n * BN + mine % (BN / 32) * 32;
-                    Piece w{pieces + (uint32_t)wj * kPieceBytes, res_bar(wj), 0u, false};
-                    if (p.out.residual && p.boxes) fetch_residual(p, w, row0, col, lane);
-                    if (!mbar_wait_for(join_bar(wj), 0, p.limit)) late = true;
-                    float z[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) z[i] = 0.f;
-                    for (int s = 0; s < p.cluster; ++s) {
-                        const uint32_t from = received + (uint32_t)(wj * p.cluster + s) * kPieceBytes;
-#pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            uint32_t f[4];
-                            lds128(from + unit128(lane, u), f[0], f[1], f[2], f[3]);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) z[4 * u + i] += __uint_as_float(f[i]);
-                        }
-                    }
-                    finish_piece<T, ACT>(p, w, z, row0, col, 0, lane, [] {});
-                    late |= w.late;
-                }
-            }
-            __syncwarp();
-            cluster_arrive();
-            cluster_wait();  // what this block has sent has arrived
-        }
-    }
-    if (warp >= 4 && lane == 0) tma_store_wait_read();
+    if (warp >= 4 && lane == 0) tma_store_wait_read<0>();
     if (late) {
         atomicCAS(p.fault, 0, kFaultLinear);
         // what is in flight (copies, products) ends in microseconds
@@ -510,26 +474,41 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
     if (warp == 2) tmem_free(tmem, 2 * BN);
 }
 
-// Joins the splits of K in their order and finishes: four elements a thread.
+// Joins the splits of K in their order and finishes.  Four elements a thread, four threads a quad with a quarter of the
+// splits each: few outputs with many splits would otherwise leave most of the machine idle (512 x 128 of 48 splits: 18 us).
 template <typename T> __global__ void __launch_bounds__(256) linear_join_kernel(const float* __restrict__ partial, const Epilogue out, int M, int N, int splits) {
-    const int quads = (N + 3) / 4;
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    __shared__ float4 part[3][64];
+    wait_for_previous();
+    const int quads = (N + 3) / 4, q = threadIdx.x & 63, quarter = threadIdx.x >> 6;
+    const long long at = (long long)blockIdx.x * 64 + q;
     const long long row = at / quads;
-    if (row >= M) return;
     const int col = (int)(at - row * quads) * 4, left = N - col;
-    float z[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool vec = (N & 3) == 0;
+    float z[4] = {0.f, 0.f, 0.f, 0.f};
+    const int per = (splits + 3) / 4, s1 = min(splits, (quarter + 1) * per);
+    if (row < M) {
+        if ((N & 3) == 0) {
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        const float* from = partial + ((long long)s * M + row) * N + col;
-        if (vec) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(from));
-            z[0] += v.x; z[1] += v.y; z[2] += v.z; z[3] += v.w;
+            for (int s = quarter * per; s < s1; ++s) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(partial + ((long long)s * M + row) * N + col));
+                z[0] += v.x; z[1] += v.y; z[2] += v.z; z[3] += v.w;
+            }
         } else {
-            for (int j = 0; j < 4; ++j)
-                if (j < left) z[j] += __ldg(from + j);
+#pragma unroll 4
+            for (int s = quarter * per; s < s1; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < left) z[j] += __ldg(partial + ((long long)s * M + row) * N + col + j);
         }
     }
+    if (quarter) part[quarter - 1][q] = make_float4(z[0], z[1], z[2], z[3]);
+    __syncthreads();
+    if (quarter || row >= M) return;
+#pragma unroll
+    for (int s = 0; s < 3; ++s) {
+        const float4 v = part[s][q];
+        z[0] += v.x; z[1] += v.y; z[2] += v.z; z[3] += v.w;
+    }
+    float b[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f};
     if (out.bias) load4(reinterpret_cast<const T*>(out.bias) + col, false, left, b);
     if (out.residual) load4(reinterpret_cast<const T*>(out.residual) + row * out.ldr + col, out.vec, left, r);
     finish4<T>(out, row, col, left, z, b, r);

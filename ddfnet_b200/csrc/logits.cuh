@@ -32,14 +32,6 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
-__device__ __forceinline__ uint4 ld_granule(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
-}
-
 template <typename T> struct Granule {
     static constexpr int N = 16 / (int)sizeof(T);
     static __device__ __forceinline__ void get(const uint4& g, float (&x)[N]) {
