@@ -103,7 +103,7 @@ struct PackPlan {
     long long ld[2], rows[2];
     int cols;
 };
-template <typename T> __global__ void __launch_bounds__(256) linear_pack_kernel(const PackPlan p) {
+template <typename T> __global__ void __launch_bounds__(256) linear_pack_kernel(const __grid_constant__ PackPlan p) {
     const int which = blockIdx.z;
     const T* src = reinterpret_cast<const T*>(p.src[which]);
     T* dst = reinterpret_cast<T*>(p.dst[which]);
@@ -133,12 +133,15 @@ struct BackPlan {
 };
 // Eight elements of a row, the first `n` of them, as they lie in memory.
 template <typename T, bool VEC> __device__ __forceinline__ uint4 load8(const T* p, int n) {
-    if constexpr (VEC) return ld_granule(p);  // (N is a multiple of eight)
-    uint32_t q[4];
+    if constexpr (VEC) {  // (N is a multiple of eight)
+        return ld_granule(p);
+    } else {
+        uint32_t q[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        q[i] = Word<T>::put(2 * i < n ? Elem<T>::load(p + 2 * i) : 0.f, 2 * i + 1 < n ? Elem<T>::load(p + 2 * i + 1) : 0.f);
-    return make_uint4(q[0], q[1], q[2], q[3]);
+        for (int i = 0; i < 4; ++i)
+            q[i] = Word<T>::put(2 * i < n ? Elem<T>::load(p + 2 * i) : 0.f, 2 * i + 1 < n ? Elem<T>::load(p + 2 * i + 1) : 0.f);
+        return make_uint4(q[0], q[1], q[2], q[3]);
+    }
 }
 template <typename T> __device__ __forceinline__ void store8(T* p, bool vec, int n, const uint4& v) {
     if (vec && n >= 8) {
@@ -150,7 +153,7 @@ template <typename T> __device__ __forceinline__ void store8(T* p, bool vec, int
             if (i < n) Elem<T>::store(p + i, Word<T>::get(q[i / 2], i % 2));
     }
 }
-template <typename T, int ACT, bool VEC> __global__ void __launch_bounds__(256) linear_back_kernel(const BackPlan p) {
+template <typename T, int ACT, bool VEC> __global__ void __launch_bounds__(256) linear_back_kernel(const __grid_constant__ BackPlan p) {
     __shared__ float sums[8][256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.x * 256 + lane * 8, left = p.N - col;
@@ -316,8 +319,8 @@ static int product(const Matrix& a, const Matrix& b, long long M, long long N, l
         p.partial = partial;
         p.boxes = N % 4 == 0;
         const cuuint64_t dims[3] = {(cuuint64_t)N, (cuuint64_t)M, (cuuint64_t)cut.splits}, strides[2] = {(cuuint64_t)N * 4, (cuuint64_t)M * N * 4};
-        const cuuint32_t box[3] = {32, 32, 1};
-        if (p.boxes && (rc = encode(&p.y, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, partial, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+        const cuuint32_t box[3] = {16, 32, 1};
+        if (p.boxes && (rc = encode(&p.y, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, partial, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B))) return rc;
     } else {
         p.boxes = addressable(out.y, out.ldy) && (!out.aux || addressable(out.aux, out.ldy)) && (!out.residual || addressable(out.residual, out.ldr));
         p.bias_vec = (reinterpret_cast<uintptr_t>(out.bias) & 15) == 0;

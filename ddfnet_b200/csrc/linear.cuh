@@ -11,7 +11,7 @@
 // results' bytes.  One persistent block an SM:
 //   warp 0     one thread loads tiles of 64 along K by TMA into a ring of stages
 //   warp 1     one thread issues the products, 128 x BN, into one of two accumulators in tensor memory
-//   warps 4-11 take the other accumulator meanwhile, in pieces of 32 x 32: a thread holds a row of it; residual and
+//   warps 4-19 take the other accumulator meanwhile, in pieces of 32 x 32: a thread holds a row of it; residual and
 //              results pass through shared memory to and from TMA, whose copies the warp does not wait for
 // BN = 256 where the tiles fill the machine: a 128 x 256 tile's operands take 96 bytes of shared memory a clock
 // at the full rate, a 128 x 128 tile's all 128.  Where they would not, smaller BN and splits of K, whose partial sums
@@ -29,14 +29,13 @@ namespace ddf {
 
 constexpr int kFaultLinear = 6;  // a wait of linear_kernel ran out
 constexpr int kTileM = 128, kTileK = 64;
-constexpr int kLinearThreads = 384, kJoinWarps = 8;
-// Shared memory: the ring of stages, and for every epilogue warp boxes of 2 KB (32 x 32 of a 2-byte type).  Wide tiles take
-// four stages and two boxes; narrower ones, which small K is for, five or six stages and four boxes: results
-// leave from two of them in turn, residuals arrive in the others.
+constexpr int kJoinWarps = 16, kLinearThreads = 128 + 32 * kJoinWarps;
+// Shared memory: the ring of stages, and for every epilogue warp one or two boxes of 2 KB (32 x 32 of a 2-byte type):
+// two where the tiles are narrow, which small K is for, so that a residual arrives while results leave.
 constexpr uint32_t kBox = 2048;
 __host__ __device__ constexpr uint32_t stage_bytes(int bn) { return (uint32_t)(kTileM + bn) * kTileK * 2; }
 __host__ __device__ constexpr int stages_of(int bn) { return bn == 256 ? 4 : bn == 128 ? 5 : 6; }
-__host__ __device__ constexpr int boxes_of(int bn) { return bn == 256 ? 2 : 4; }
+__host__ __device__ constexpr int boxes_of(int bn) { return bn == 256 ? 1 : 2; }
 __host__ __device__ constexpr uint32_t linear_shared(int bn) {
     return stages_of(bn) * stage_bytes(bn) + kJoinWarps * boxes_of(bn) * kBox + 1024 + 512;
 }
@@ -169,55 +168,60 @@ __device__ __forceinline__ void tile_of(const LinearPlan& p, int item, int& m, i
 
 // What an epilogue warp needs to finish a piece of 32 rows x 32 columns, one row a lane.
 struct Piece {
-    uint32_t stage;      // its boxes: `outs` for results, then `ins` for residuals
-    uint32_t bar;        // of the first residual box's copy; the second's follows
-    int outs, ins;
-    int out, in;         // the next of each
-    uint32_t phases;     // of the residual boxes' barriers, a bit each
+    uint32_t box;    // its boxes
+    uint32_t bar;    // of the residual's copy
+    int outs, out;   // boxes for results, and the next of them
+    uint32_t in;     // the residual's box: one of its own, or the results'
+    uint32_t phase;  // of the residual's barrier
     bool late;
 };
-// 16-byte unit u of row `lane` of a box of 64-byte rows (64-byte swizzle) or 128-byte rows (128-byte swizzle).
+// 16-byte unit u of row `lane` of a box of 64-byte rows (64-byte swizzle).
 __device__ __forceinline__ uint32_t unit64(int lane, int u) { return lane * 64 + ((u ^ (lane >> 1 & 3)) * 16); }
-__device__ __forceinline__ uint32_t unit128(int lane, int u) { return lane * 128 + ((u ^ (lane & 7)) * 16); }
 
-__device__ __forceinline__ void fetch_residual(const LinearPlan& p, const Piece& w, int box, int row0, int col, int lane) {
+__device__ __forceinline__ void fetch_residual(const LinearPlan& p, const Piece& w, int row0, int col, int lane) {
     if (lane == 0) {
-        const uint32_t bar = w.bar + 8u * box;
-        mbar_arrive_expect_tx(bar, kBox);
-        tma_load_2d(w.stage + (w.outs + box) * kBox, &p.r, col, row0, bar);
+        if (w.in == w.box) tma_store_wait_read<0>();  // (a box for both)
+        mbar_arrive_expect_tx(w.bar, kBox);
+        tma_load_2d(w.in, &p.r, col, row0, w.bar);
     }
 }
-// Waits for the residual of the next piece; its box's address.
-__device__ __forceinline__ uint32_t await_residual(const LinearPlan& p, Piece& w) {
-    if (!w.late && !mbar_wait_for(w.bar + 8u * w.in, w.phases >> w.in & 1u, p.limit)) w.late = true;
-    w.phases ^= 1u << w.in;
-    return w.stage + (w.outs + w.in) * kBox;
+__device__ __forceinline__ void await_residual(const LinearPlan& p, Piece& w) {
+    if (!w.late && !mbar_wait_for(w.bar, w.phase, p.limit)) w.late = true;
+    w.phase ^= 1u;
 }
-// Before a box for results is written again.
-__device__ __forceinline__ void await_out(const Piece& w, int lane) {
+// A box for results, free to be written.
+__device__ __forceinline__ uint32_t next_out(Piece& w, int lane) {
     if (lane == 0) {
         if (w.outs > 1) tma_store_wait_read<1>();
         else tma_store_wait_read<0>();
     }
     __syncwarp();
+    const uint32_t to = w.box + w.out * kBox;
+    if (++w.out == w.outs) w.out = 0;
+    return to;
 }
 
-// z: the lane's row of the product.  `next(box)`: called when the residual in `box` is in registers.
+// z: the lane's row of the product.  `next`: called when the residual's box may be filled again.
 template <typename T, int ACT, typename Next>
 __device__ __forceinline__ void finish_piece(const LinearPlan& p, Piece& w, float (&z)[32], int row0, int col, int split, int lane, Next next) {
     const Epilogue& e = p.out;
     if (p.partial) {
         if (p.boxes) {
-            if (lane == 0) tma_store_wait_read<0>();
-            __syncwarp();
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                sts128(w.stage + unit128(lane, u), __float_as_uint(z[4 * u]), __float_as_uint(z[4 * u + 1]), __float_as_uint(z[4 * u + 2]), __float_as_uint(z[4 * u + 3]));
-            fence_async();
-            __syncwarp();
-            if (lane == 0) {
-                tma_store_3d(&p.y, w.stage, col, row0, split);
-                tma_store_commit();
+            for (int h = 0; h < 2; ++h) {
+                if (col + 16 * h >= p.N) break;
+                const uint32_t to = next_out(w, lane);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float* f = z + 16 * h + 4 * u;
+                    sts128(to + unit64(lane, u), __float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+                }
+                fence_async();
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_3d(&p.y, to, col + 16 * h, row0, split);
+                    tma_store_commit();
+                }
             }
             return;
         }
@@ -239,22 +243,23 @@ __device__ __forceinline__ void finish_piece(const LinearPlan& p, Piece& w, floa
             }
         }
         uint32_t r[16];
+        const bool own = w.in != w.box;  // the residual has a box of its own
         if (e.residual) {
-            const uint32_t from = await_residual(p, w);
+            await_residual(p, w);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) lds128v(from + unit64(lane, u), r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
-            fence_async();  // these reads come before the next copy's writes: the warp's barrier alone does not see to that
-            __syncwarp();
-            next(w.in);
-            if (++w.in == w.ins) w.in = 0;
+            for (int u = 0; u < 4; ++u) lds128v(w.in + unit64(lane, u), r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
+            if (own) {
+                fence_async();  // these reads come before the next copy's writes: the warp's barrier alone does not see to that
+                __syncwarp();
+                next();
+            }
         }
         const auto add = [&] {
 #pragma unroll
             for (int i = 0; i < 32; ++i) z[i] += Word<T>::get(r[i / 2], i % 2);
         };
         const auto store = [&](const CUtensorMap* map) {
-            const uint32_t to = w.stage + w.out * kBox;
-            await_out(w, lane);
+            const uint32_t to = next_out(w, lane);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 sts128(to + unit64(lane, u), Word<T>::put(z[8 * u], z[8 * u + 1]), Word<T>::put(z[8 * u + 2], z[8 * u + 3]),
@@ -265,7 +270,6 @@ __device__ __forceinline__ void finish_piece(const LinearPlan& p, Piece& w, floa
                 tma_store_2d(map, to, col, row0);
                 tma_store_commit();
             }
-            if (++w.out == w.outs) w.out = 0;
         };
         if (e.residual && !e.after) add();
         if (e.aux) store(&p.aux);
@@ -273,40 +277,47 @@ __device__ __forceinline__ void finish_piece(const LinearPlan& p, Piece& w, floa
         for (int i = 0; i < 32; ++i) z[i] = act_value<ACT>(z[i]);
         if (e.residual && e.after) add();
         store(&p.y);
+        if (e.residual && !own) next();
         return;
     }
-    // rows that TMA cannot address: turned in shared memory, a column a lane
+    // rows that TMA cannot address: turned in shared memory, sixteen columns at a time, two rows a warp's access
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-        sts128(w.stage + unit128(lane, u), __float_as_uint(z[4 * u]), __float_as_uint(z[4 * u + 1]), __float_as_uint(z[4 * u + 2]), __float_as_uint(z[4 * u + 3]));
-    __syncwarp();
-    const int c = col + lane, rows = min(32, p.M - row0);
-    if (c < p.N) {
-        const float bias = !p.partial && e.bias ? Elem<T>::load(reinterpret_cast<const T*>(e.bias) + c) : 0.f;
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float* f = z + 16 * h + 4 * u;
+            sts128(w.box + unit64(lane, u), __float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        }
+        __syncwarp();
+        const int in = lane & 15, c = col + 16 * h + in, rows = min(32, p.M - row0);
+        if (c < p.N) {
+            const float bias = !p.partial && e.bias ? Elem<T>::load(reinterpret_cast<const T*>(e.bias) + c) : 0.f;
 #pragma unroll 4
-        for (int i = 0; i < rows; ++i) {
-            const long long row = row0 + i;
-            float v = ldsf(w.stage + unit128(i, lane >> 2) + (lane & 3) * 4);
-            if (p.partial) {
-                p.partial[((long long)split * p.M + row) * p.N + c] = v;
-            } else {
-                const float r = e.residual ? Elem<T>::load(reinterpret_cast<const T*>(e.residual) + row * e.ldr + c) : 0.f;
-                v += bias;
-                if (!e.after) v += r;
-                if (e.aux) Elem<T>::store(reinterpret_cast<T*>(e.aux) + row * e.ldy + c, v);
-                v = act_value<ACT>(v);
-                if (e.after) v += r;
-                Elem<T>::store(reinterpret_cast<T*>(e.y) + row * e.ldy + c, v);
+            for (int i = lane >> 4; i < rows; i += 2) {
+                const long long row = row0 + i;
+                float v = ldsf(w.box + unit64(i, in >> 2) + (in & 3) * 4);
+                if (p.partial) {
+                    p.partial[((long long)split * p.M + row) * p.N + c] = v;
+                } else {
+                    const float r = e.residual ? Elem<T>::load(reinterpret_cast<const T*>(e.residual) + row * e.ldr + c) : 0.f;
+                    v += bias;
+                    if (!e.after) v += r;
+                    if (e.aux) Elem<T>::store(reinterpret_cast<T*>(e.aux) + row * e.ldy + c, v);
+                    v = act_value<ACT>(v);
+                    if (e.after) v += r;
+                    Elem<T>::store(reinterpret_cast<T*>(e.y) + row * e.ldy + c, v);
+                }
             }
         }
+        __syncwarp();
     }
-    __syncwarp();
 }
 
 template <typename T, int BN, bool AT, bool BT, int ACT>
 __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_constant__ LinearPlan p) {
     constexpr uint32_t kA = kTileM * kTileK * 2, kStage = stage_bytes(BN);
     constexpr int kStages = stages_of(BN), kBoxes = boxes_of(BN);
+    constexpr int kGroups = BN / 32 < kJoinWarps / 4 ? BN / 32 : kJoinWarps / 4;  // of four warps, each with its columns
     extern __shared__ unsigned char linear_raw[];
     const uint32_t base = (smem_u32(linear_raw) + 1023u) & ~1023u;
     const uint32_t pieces = base + kStages * kStage, bars = pieces + kJoinWarps * kBoxes * kBox;
@@ -314,8 +325,8 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
     const auto empty = [&](int s) { return bars + 8u * (kStages + s); };
     const auto acc_full = [&](int s) { return bars + 8u * (2 * kStages + s); };
     const auto acc_empty = [&](int s) { return bars + 8u * (2 * kStages + 2 + s); };
-    const auto res_bar = [&](int w) { return bars + 8u * (2 * kStages + 4 + 2 * w); };
-    const uint32_t tmem_word = bars + 8u * (2 * kStages + 4 + 2 * kJoinWarps);
+    const auto res_bar = [&](int w) { return bars + 8u * (2 * kStages + 4 + w); };
+    const uint32_t tmem_word = bars + 8u * (2 * kStages + 4 + kJoinWarps);
     const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be the warp's)
     const int items = p.tiles_m * p.tiles_n * p.splits;
     const int all_steps = (p.K + kTileK - 1) / kTileK;
@@ -328,12 +339,9 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(acc_full(s), 1);
-            mbar_init(acc_empty(s), kJoinWarps);
+            mbar_init(acc_empty(s), 4 * kGroups);
         }
-        for (int w = 0; w < kJoinWarps; ++w) {
-            mbar_init(res_bar(w), 1);
-            mbar_init(res_bar(w) + 8u, 1);
-        }
+        for (int w = 0; w < kJoinWarps; ++w) mbar_init(res_bar(w), 1);
         mbar_fence_init();
         tma_prefetch_map(&p.a);
         tma_prefetch_map(&p.b);
@@ -406,18 +414,18 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
             }
             if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
         }
-    } else if (warp >= 4) {
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
-        const int c0 = half * (BN / 2), c1 = c0 + BN / 2;
+    } else if (warp >= 4 && warp < 4 + 4 * kGroups) {
+        const int quarter = warp & 3, group = (warp - 4) >> 2;
+        const int c0 = group * (BN / kGroups), c1 = c0 + BN / kGroups;
         const bool residual = p.out.residual && p.boxes && !p.partial;
-        const int ins = residual ? kBoxes / 2 : 0;
-        Piece w{pieces + (uint32_t)(warp - 4) * kBoxes * kBox, res_bar(warp - 4), residual ? kBoxes / 2 : 2, ins, 0, 0, 0u, false};
-        // the residuals' copies run `ins` pieces ahead
+        const uint32_t box = pieces + (uint32_t)(warp - 4) * kBoxes * kBox;
+        Piece w{box, res_bar(warp - 4), residual ? 1 : kBoxes, 0, box + (kBoxes - 1) * kBox, 0u, false};
+        // the residual's copy runs one piece ahead
         int fetch_item = blockIdx.x, fetch_c = c0, fetch_m = 0, fetch_n = 0, unused;
         if (residual && fetch_item < items) tile_of(p, fetch_item, fetch_m, fetch_n, unused);
-        const auto next = [&](int box) {
+        const auto next = [&] {
             if (fetch_item >= items) return;
-            fetch_residual(p, w, box, fetch_m * kTileM + quarter * 32, fetch_n * BN + fetch_c, lane);
+            fetch_residual(p, w, fetch_m * kTileM + quarter * 32, fetch_n * BN + fetch_c, lane);
             fetch_c += 32;
             if (fetch_c == c1) {
                 fetch_c = c0;
@@ -425,7 +433,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
                 if (fetch_item < items) tile_of(p, fetch_item, fetch_m, fetch_n, unused);
             }
         };
-        for (int box = 0; box < ins; ++box) next(box);
+        if (residual) next();
         int acc = 0;
         uint32_t acc_phase = 0;
         for (int item = blockIdx.x; item < items; item += gridDim.x) {
@@ -453,8 +461,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
                 } else if (residual) {  // nothing to finish, but its copy is on the way
                     await_residual(p, w);
                     __syncwarp();
-                    next(w.in);
-                    if (++w.in == w.ins) w.in = 0;
+                    next();
                 }
             }
             if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
