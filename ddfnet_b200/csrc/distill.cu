@@ -31,7 +31,6 @@ extern std::atomic<unsigned long long> g_launches;
 int device_facts(int* sm_count, int** fault, int* index);
 
 constexpr int kStats = 8;                     // floats a row between forward and backward
-constexpr int kSliceBytes = 64 * 1024;        // of a block's share of the row in shared memory: three blocks an SM
 constexpr int kWarpElements = 1024;           // a row (with what its first granule holds before it) in a warp
 constexpr int kCountBlocks = 128;
 enum { kLoss = 1, kGrad = 2 };
@@ -47,6 +46,7 @@ struct DistillPlan {
     int V, K, slices, per, n_counts;
     int values_dtype, wide_indices;
     float c, T, scale;
+    int* fault;
 };
 
 // One row's softmaxes over the buckets, in base 2:  log2 p_k = (a_k - ra) log2(e) - la,
@@ -75,40 +75,40 @@ __device__ __forceinline__ float log2_total(float sum, int ties) {
     return log1pf(sum + (float)(ties - 1)) * kLog2e;
 }
 
-// The bucket softmaxes of a row from its entries in shared memory; called by whole warps, each for itself.
-__device__ __forceinline__ Row buckets(const float* a, const float* s, int K, float rest, const Online& others, float c) {
+// The bucket softmaxes of a row from its entries in shared memory: the teacher's, and the student's with what the others
+// sum to.  Called by one whole warp.
+__device__ __forceinline__ void teacher_buckets(Row& r, const float* a, int K, float rest) {
     const int lane = threadIdx.x & 31;
-    float ra = rest, ms = neg_inf();
-    for (int k = lane; k < K; k += 32) {
-        ra = max_nan(ra, a[k]);
-        ms = max_nan(ms, s[k]);
-    }
-    Row r;
+    float ra = rest;
+    for (int k = lane; k < K; k += 32) ra = max_nan(ra, a[k]);
     r.ra = warp_max_nan(ra);
-    r.m = max_nan(warp_max_nan(ms), others.m);
-    if (r.m == neg_inf()) r.m = 0.f;
     const float base = r.ra == neg_inf() ? 0.f : r.ra;
     r.rest_a = (rest - base) * kLog2e;
+    float sum = 0.f;
+    int ties = 0;
+    auto add = [&](float e) { if (e == 0.f) ++ties; else sum += ex2(e); };
+    for (int k = lane; k < K; k += 32) add((a[k] - base) * kLog2e);
+    if (lane == 0) add(r.rest_a);
+    // (without any tie all entries are -inf or one is NaN: the logarithm is then 0, or NaN)
+    r.la = log2_total(warp_sum(sum), max(1, __reduce_add_sync(~0u, ties)));
+}
+__device__ __forceinline__ void student_buckets(Row& r, const float* s, int K, const Online& others, float c) {
+    const int lane = threadIdx.x & 31;
+    float m = others.m;
+    for (int k = lane; k < K; k += 32) m = max_nan(m, s[k]);
+    r.m = warp_max_nan(m);
+    if (r.m == neg_inf()) r.m = 0.f;
     r.rest_b = others.s == 0.f ? neg_inf() : log2f(others.s) + (others.ref - r.m) * c;
     float top = r.rest_b;
     for (int k = lane; k < K; k += 32) top = max_nan(top, (s[k] - r.m) * c);
     r.top = warp_max_nan(top);
     if (r.top == neg_inf()) r.top = 0.f;
-    float sum_a = 0.f, sum_b = 0.f;
-    int ties_a = 0, ties_b = 0;
-    auto add = [&](float ea, float eb) {
-        if (ea == 0.f) ++ties_a; else sum_a += ex2(ea);
-        if (eb == 0.f) ++ties_b; else sum_b += ex2(eb);
-    };
-    for (int k = lane; k < K; k += 32) add((a[k] - base) * kLog2e, (s[k] - r.m) * c - r.top);
-    if (lane == 0) add(r.rest_a, r.rest_b - r.top);
-    // (without any tie all entries are -inf or one is NaN: the logarithm is then 0, or NaN)
-    ties_a = max(1, __reduce_add_sync(~0u, ties_a));
-    ties_b = max(1, __reduce_add_sync(~0u, ties_b));
-    r.la = log2_total(warp_sum(sum_a), ties_a);
-    r.lb = log2_total(warp_sum(sum_b), ties_b);
-    r.repeated = false;
-    return r;
+    float sum = 0.f;
+    int ties = 0;
+    auto add = [&](float e) { if (e == 0.f) ++ties; else sum += ex2(e); };
+    for (int k = lane; k < K; k += 32) add((s[k] - r.m) * c - r.top);
+    if (lane == 0) add(r.rest_b - r.top);
+    r.lb = log2_total(warp_sum(sum), max(1, __reduce_add_sync(~0u, ties)));
 }
 
 // p log(p/q) - p + q of a bucket, and q - p, from the exponents log2 p and log2 q.
@@ -209,13 +209,12 @@ __device__ __forceinline__ Others others_of(const Row& r, float g) {
     return o;
 }
 template <int N> __device__ __forceinline__ void others_grad(const Others& o, float c, float (&x)[N]) {
-    const unsigned long long m2 = f2_pack(-o.m, -o.m), c2 = f2_pack(c, c), s2 = f2_pack(-o.shift, -o.shift);
+    const unsigned long long m2 = f2_pack(-o.m, -o.m), c2 = f2_pack(c, c), s2 = f2_pack(-o.shift, -o.shift), f2 = f2_pack(o.factor, o.factor);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
         float a, b;
         f2_unpack(f2_fma(f2_add(f2_pack(x[i], x[i + 1]), m2), c2, s2), a, b);
-        x[i] = o.factor * ex2(a);
-        x[i + 1] = o.factor * ex2(b);
+        f2_unpack(f2_mul(f2_pack(ex2(a), ex2(b)), f2), x[i], x[i + 1]);
     }
 }
 
@@ -234,11 +233,10 @@ __device__ __forceinline__ void store_granule(const Run<T>& run, T* out, int g, 
     }
 }
 
-template <typename T> __device__ __forceinline__ float largest(const float (&x)[Granule<T>::N]) {
-    float m = x[0];
-#pragma unroll
-    for (int i = 1; i < Granule<T>::N; ++i) m = max_nan(m, x[i]);
-    return m;
+// Bits of granule g's elements in a bitmap of the run's elements.
+template <typename T> __device__ __forceinline__ uint32_t granule_bits(const uint32_t* bits, int g) {
+    if constexpr (Granule<T>::N == 8) return reinterpret_cast<const unsigned char*>(bits)[g];
+    else return bits[g >> 3] >> (g & 7) * 4 & 15u;
 }
 template <typename T> __device__ __forceinline__ void mask(float (&x)[Granule<T>::N], uint32_t bits) {
 #pragma unroll
@@ -299,12 +297,13 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_warp_kernel(const __gr
             if (g >= run.granules) break;
             float v[N];
             Granule<T>::get(raw[u], v);
-            const uint32_t out = (bits[g * N >> 5] >> (g * N & 31) & ((1u << N) - 1u)) | run.outside(g);
+            const uint32_t out = granule_bits<T>(bits, g) | run.outside(g);
             if (out) mask<T>(v, out);
-            others.add(v, largest<T>(v), p.c);
+            others.add(v, p.c);
         }
         others = warp_merge(others, p.c);
-        r = buckets(a, s, K, rest, others, p.c);
+        teacher_buckets(r, a, K, rest);
+        student_buckets(r, s, K, others, p.c);
         r.repeated = repeated;
         const float loss = row_loss(r, a, s, K, p.c, p.T);
         if (lane == 0) {
@@ -341,16 +340,36 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_warp_kernel(const __gr
 }
 
 // ------------------------------------------------------------------ a row in a block or a cluster
-constexpr int kRowThreads = 256;
+// 16 bytes to the place that `at` is in block `rank` of the cluster, counted by the barrier that `bar` is there.
+__device__ __forceinline__ void send_to_block(uint32_t at, uint32_t bar, uint32_t rank, const float4& v) {
+    uint32_t there, bar_there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar_there) : "r"(bar), "r"(rank));
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(there), "f"(v.x), "f"(v.y), "f"(v.z),
+                 "f"(v.w), "r"(bar_there)
+                 : "memory");
+}
+
+// RESIDENT: the slice lies in shared memory, brought there by bulk copies that start before anything else and arrive
+// while the entries are read.  Otherwise (classes that fit no cluster's shared memory) it is read from memory by each pass.
+constexpr int kRowThreads = 512;
 
 template <typename T, int MODE, bool RESIDENT>
-__global__ void __launch_bounds__(kRowThreads) distill_block_kernel(const __grid_constant__ DistillPlan p) {
+__global__ void __launch_bounds__(kRowThreads, 3) distill_block_kernel(const __grid_constant__ DistillPlan p) {
     constexpr int N = Granule<T>::N;
-    constexpr int NT = kRowThreads, UNROLL = 4;
+    constexpr int NT = kRowThreads;
+    static_assert(NT >= kMaxTop && kChunk % NT == 0, "a thread for each entry; a chunk is whole turns of the block");
+    constexpr int TURNS = kChunk / NT;
     extern __shared__ __align__(16) unsigned char raw_shared[];
     __shared__ __align__(16) int cls[kMaxTop];
     __shared__ float a[kMaxTop], s[kMaxTop];
-    __shared__ Online room[NT / 32], peers[8];
+    __shared__ Online room[NT / 32];
+    __shared__ __align__(16) float4 peers[8];
+    __shared__ unsigned long long peers_bar;
+    __shared__ Arrival arrival;
+    __shared__ Row shared_row;
+    __shared__ Others shared_others;
+    __shared__ float shared_factor;
     const int tid = threadIdx.x;
     const int K = p.K;
     const long long row = blockIdx.x / (unsigned)p.slices;
@@ -360,7 +379,14 @@ __global__ void __launch_bounds__(kRowThreads) distill_block_kernel(const __grid
     const Run<T> run(x + v0, min(p.per, p.V - v0));
     uint4* copy = reinterpret_cast<uint4*>(raw_shared);
     uint32_t* bits = reinterpret_cast<uint32_t*>(raw_shared + (RESIDENT ? (size_t)run.granules * 16 : 0));
+    bool late = false;
 
+    // ---- while the slice arrives: the entries, the teacher's softmax
+    if (tid == 0) {
+        if constexpr ((MODE & kLoss) != 0) mbar_init(smem_u32(&peers_bar), 1);
+        if constexpr (RESIDENT) fetch_run(run, copy, arrival);
+        else mbar_fence_init();
+    }
     if constexpr ((MODE & kLoss) != 0) {
         if (p.slices > 1) cooperative_groups::this_cluster().barrier_arrive();
         for (int i = tid; i < (run.granules * N + 31) / 32; i += NT) bits[i] = 0;
@@ -371,6 +397,12 @@ __global__ void __launch_bounds__(kRowThreads) distill_block_kernel(const __grid
         cls[tid] = mine;
         a[tid] = mine < 0 ? neg_inf() : entry_value(p.values, row * K + tid, p.values_dtype) / p.T;
         s[tid] = mine < 0 ? neg_inf() : Elem<T>::load(x + mine);
+    }
+    if constexpr ((MODE & kGrad) != 0) {
+        if (tid >= NT - 32) {
+            const float f = grad_factor(p, row);
+            if (tid == NT - 1) shared_factor = f;
+        }
     }
     const bool any = __syncthreads_or(mine >= 0);
     const float rest = any && p.rest ? __ldg(p.rest + row) : neg_inf();
@@ -383,10 +415,13 @@ __global__ void __launch_bounds__(kRowThreads) distill_block_kernel(const __grid
                 const uint32_t at = (uint32_t)(mine - v0 + run.phase);
                 atomicOr(bits + (at >> 5), 1u << (at & 31u));
             }
-            for (int i = 0; i < tid; ++i) twice |= cls[i] == mine;
+            for (int i = 0; i < tid; i += 4) {
+                const int4 c = *reinterpret_cast<const int4*>(cls + i);
+                twice |= c.x == mine || (i + 1 < tid && c.y == mine) || (i + 2 < tid && c.z == mine) || (i + 3 < tid && c.w == mine);
+            }
         }
-        if (tid == 0) atomicOr(bits, run.outside(0));
-        if (tid == 1) atomicOr(bits + ((run.granules - 1) * N >> 5), run.outside(run.granules - 1) << ((run.granules - 1) * N & 31));
+        if (tid == NT - 1) atomicOr(bits, run.outside(0));
+        if (tid == NT - 2) atomicOr(bits + ((run.granules - 1) * N >> 5), run.outside(run.granules - 1) << ((run.granules - 1) * N & 31));
         repeated = __syncthreads_or(twice);
     } else {
         r = get_stats(p.stats + row * kStats, rest);
@@ -397,63 +432,65 @@ __global__ void __launch_bounds__(kRowThreads) distill_block_kernel(const __grid
         if (tid < K) mine = cls[tid];
     }
 
+    // ---- the sum over the others; then one warp finds what the whole block needs
     if constexpr ((MODE & kLoss) != 0) {
+        if (tid < 32) teacher_buckets(r, a, K, rest);
         Online others = Online::none();
-        for (int g0 = tid; g0 < run.granules; g0 += NT * UNROLL) {
-            uint4 raw[UNROLL];
+        for (int c = 0; c * kChunk < run.granules; ++c) {
+            if (RESIDENT && !late) late = !await_chunk(arrival, c);
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u)
-                if (g0 + u * NT < run.granules) raw[u] = run.load(g0 + u * NT);
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                const int g = g0 + u * NT;
+            for (int u = 0; u < TURNS; ++u) {
+                const int g = c * kChunk + u * NT + tid;
                 if (g >= run.granules) break;
-                if constexpr (RESIDENT) copy[g] = raw[u];
                 float v[N];
-                Granule<T>::get(raw[u], v);
-                const uint32_t out = bits[g * N >> 5] >> (g * N & 31) & ((1u << N) - 1u);
+                Granule<T>::get(RESIDENT ? copy[g] : run.load(g), v);
+                const uint32_t out = granule_bits<T>(bits, g);
                 if (out) mask<T>(v, out);
-                others.add(v, largest<T>(v), p.c);
+                others.add(v, p.c);
             }
         }
-        others = block_merge<NT / 32>(others, p.c, room);
-        if (p.slices > 1) {
-            auto cluster = cooperative_groups::this_cluster();
-            cluster.barrier_wait();  // every block of the cluster runs
-            if (tid < p.slices) *cluster.map_shared_rank(&peers[rank], tid) = others;
-            cluster.sync();
-            others = Online::none();
-            for (int i = 0; i < p.slices; ++i) others.merge(peers[i], p.c);
-        }
-        r = buckets(a, s, K, rest, others, p.c);
-        r.repeated = repeated;
-        if (rank == 0 && tid < 32) {
-            const float loss = row_loss(r, a, s, K, p.c, p.T);
-            if (tid == 0) {
-                p.losses[row] = loss;
-                if (p.stats) put_stats(p.stats + row * kStats, r);
+        const Online w = warp_merge(others, p.c);
+        if ((tid & 31) == 0) room[tid >> 5] = w;
+        if (p.slices > 1) cooperative_groups::this_cluster().barrier_wait();  // every block of the cluster has its barrier
+        __syncthreads();
+        if (tid < 32) {
+            others = warp_merge(tid < NT / 32 ? room[tid] : Online::none(), p.c);
+            if (p.slices > 1) {
+                // to every block of the cluster, with word to the one that waits there: no barrier of all its threads
+                const uint32_t bar = smem_u32(&peers_bar);
+                if (tid == 0) mbar_arrive_expect_tx(bar, (uint32_t)p.slices * 16u);
+                __syncwarp();
+                if (tid < p.slices) send_to_block(smem_u32(&peers[rank]), bar, tid, make_float4(others.m, others.ref, others.s, 0.f));
+                if (!late) late = !mbar_wait(bar, 0);
+                __syncwarp();
+                const float4 q = tid < p.slices ? peers[tid] : make_float4(neg_inf(), 0.f, 0.f, 0.f);
+                others = warp_merge(Online{q.x, q.y, q.z}, p.c);
             }
+            student_buckets(r, s, K, others, p.c);
+            r.repeated = repeated;
         }
     }
     if constexpr ((MODE & kGrad) != 0) {
+        if (tid < 32) {
+            const Others o = others_of(r, shared_factor);
+            if (tid == 0) {
+                shared_row = r;
+                shared_others = o;
+            }
+        }
+        __syncthreads();
         T* out = reinterpret_cast<T*>(p.grad) + row * p.V;
         const bool even = (reinterpret_cast<unsigned long long>(out + v0) & 15ull) == (reinterpret_cast<unsigned long long>(x + v0) & 15ull);
-        const float f = grad_factor(p, row);
-        const Others o = others_of(r, f);
-        const bool counted = r.counted();
-        for (int g0 = tid; g0 < run.granules; g0 += NT * UNROLL) {
-            uint4 raw[UNROLL];
-            if constexpr (!RESIDENT) {
+        const Others o = shared_others;
+        const bool counted = shared_row.counted();
+        for (int c = 0; c * kChunk < run.granules; ++c) {
+            if (RESIDENT && MODE == kGrad && !late) late = !await_chunk(arrival, c);
 #pragma unroll
-                for (int u = 0; u < UNROLL; ++u)
-                    if (g0 + u * NT < run.granules) raw[u] = run.load(g0 + u * NT);
-            }
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                const int g = g0 + u * NT;
+            for (int u = 0; u < TURNS; ++u) {
+                const int g = c * kChunk + u * NT + tid;
                 if (g >= run.granules) break;
                 float v[N];
-                Granule<T>::get(RESIDENT ? copy[g] : raw[u], v);
+                Granule<T>::get(RESIDENT ? copy[g] : run.load(g), v);
                 others_grad(o, p.c, v);
                 if (!counted) {
 #pragma unroll
@@ -463,8 +500,28 @@ __global__ void __launch_bounds__(kRowThreads) distill_block_kernel(const __grid
             }
         }
         __syncthreads();  // the listed classes' gradients go over what the loop has put there
-        if (counted && mine >= v0 && mine < v0 + run.len)
-            Elem<T>::store(out + mine, f * q_minus_p(log2_p(r, a[tid]), log2_q(r, s[tid], p.c)));
+        if (counted && mine >= v0 && mine < v0 + run.len) {
+            const Row q = shared_row;
+            Elem<T>::store(out + mine, shared_factor * q_minus_p(log2_p(q, a[tid]), log2_q(q, s[tid], p.c)));
+        }
+    }
+    if constexpr ((MODE & kLoss) != 0) {
+        if (rank == 0 && tid < 32) {
+            const float loss = row_loss(r, a, s, K, p.c, p.T);
+            if (tid == 0) {
+                p.losses[row] = loss;
+                if (p.stats) put_stats(p.stats + row * kStats, r);
+            }
+        }
+    }
+    if (late) give_up(p.fault);
+    if constexpr ((MODE & kLoss) != 0) {
+        // no block ends while another may still send to it (each of the others has sent, unless a wait ran out)
+        __syncwarp();
+        if (p.slices > 1) {
+            asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+            asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        }
     }
 }
 
@@ -536,15 +593,12 @@ static int distill_launch(DistillPlan p, int sm_count, cudaStream_t st) {
         const long long row_bytes = (long long)p.V * ES;
         long long slices = 1;
         if (MODE == kGrad) {
-            // blocks on their own: 32 KB keep one for some microseconds, a sixteenth of that where there are few rows
-            slices = (row_bytes + 32767) / 32768;
+            // blocks on their own, down to 4 KB each where there are few rows
+            slices = (row_bytes + 64 + kResidentBytes - 1) / kResidentBytes;
             while (p.rows * slices < 2 * sm_count && row_bytes / slices > 4096) slices *= 2;
         } else {
             // a cluster for each row: slices that fit shared memory, or, with few rows, more of them
-            while (slices < 8 && ((MODE == (kLoss | kGrad) && row_bytes / slices + 64 > kSliceBytes) ||
-                                  p.V / 8 / slices > kSliceBytes ||  // the bitmap
-                                  (p.rows * slices < 2 * sm_count && row_bytes / slices > 8192)))
-                slices *= 2;
+            while (slices < 8 && (row_bytes / slices + 64 > kResidentBytes || (p.rows * slices < 2 * sm_count && row_bytes / slices > 8192))) slices *= 2;
         }
         long long per = (p.V + slices - 1) / slices;
         per = (per + 7) / 8 * 8;  // granules of the slices keep the row's phase
@@ -553,7 +607,7 @@ static int distill_launch(DistillPlan p, int sm_count, cudaStream_t st) {
         p.per = (int)per;
         p.slices = (int)slices;
         const size_t granules = (size_t)(per + N - 1) / N + 1;
-        const bool resident = MODE == (kLoss | kGrad) && granules * 16 <= kSliceBytes + 64;
+        const bool resident = granules <= kResidentGranules;
         const size_t bytes = (resident ? granules * 16 : 0) + (MODE & kLoss ? (granules * N + 31) / 32 * 4 : 0);
         if (bytes > 200 * 1024) return DDF_B200_E_ARGUMENT;
         cudaLaunchConfig_t cfg = {};
@@ -607,7 +661,7 @@ static int distill_check(const ddf_b200_distill_args* q, DistillPlan& p, int* sm
     p.stride = q->row_stride; p.rows = q->rows; p.V = (int)q->classes; p.K = q->k;
     p.values_dtype = q->values_dtype; p.wide_indices = q->wide_indices;
     p.c = (float)(1.4426950408889634 / q->temperature); p.T = T;
-    p.scale = 1.f; p.slices = 1;
+    p.scale = 1.f; p.slices = 1; p.fault = fault;
     return 0;
 }
 

@@ -70,28 +70,79 @@ template <typename T> struct Run {
     }
 };
 
-// Sum of 2^((x - m) c) over the elements x so far, m the largest of them.  Nothing yet, or nothing above
-// -inf: m = -inf, s = 0, and `ref`, which stands for m in differences, 0.  A NaN or +inf makes s NaN for good.
+// A run's granules on their way to shared memory by bulk copies, all of them at once: no registers and no turns of a
+// loop between a row's bytes and the memory that delivers them.  A chunk is kChunk granules, with a barrier each.
+constexpr int kChunk = 1024;
+constexpr int kResidentBytes = 64 * 1024;                        // of a row that a block keeps: three blocks an SM
+constexpr int kResidentGranules = kResidentBytes / 16 + 1;       // (a run may start inside a granule)
+constexpr int kChunks = (kResidentGranules + kChunk - 1) / kChunk;
+constexpr int kFaultLogits = 7;                                  // a wait for a chunk ran out
+struct Arrival {
+    unsigned long long bar[kChunks];
+};
+// One thread, before the block's first barrier.
+template <typename T> __device__ __forceinline__ void fetch_run(const Run<T>& run, void* to, Arrival& a) {
+    const uint32_t bar = smem_u32(a.bar), dst = smem_u32(to);
+    for (int c = 0; c < kChunks; ++c) mbar_init(bar + 8u * c, 1);
+    mbar_fence_init();
+    for (int c = 0, g = 0; g < run.granules; ++c, g += kChunk) {
+        const uint32_t bytes = (uint32_t)min(kChunk, run.granules - g) * 16u;
+        mbar_arrive_expect_tx(bar + 8u * c, bytes);
+        bulk_g2s(dst + (uint32_t)g * 16u, run.base + (long long)g * 16, bytes, bar + 8u * c);
+    }
+}
+// False where the wait ran out; the caller carries on without waiting again, and ends with give_up().
+__device__ __forceinline__ bool await_chunk(Arrival& a, int c) { return mbar_wait(smem_u32(a.bar) + 8u * c, 0); }
+// Records the fault, and leaves the copies time to land before the block's shared memory is another's.
+__device__ __forceinline__ void give_up(int* fault) {
+    atomicCAS(fault, 0, kFaultLogits);
+    for (int i = 0; i < 100; ++i) __nanosleep(100000);
+}
+
+template <int N> __device__ __forceinline__ float largest(const float (&x)[N]) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = max_nan(m, x[i]);
+    return m;
+}
+// Over the warp, in one instruction; NaN if one is.
+__device__ __forceinline__ float warp_max_nan(float v) {
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// Sum of 2^((x - m) c) over the elements x so far, m one of them, less than 8 / c below the largest.  Nothing yet, or
+// nothing above -inf: m = -inf, s = 0, and `ref`, which stands for m in differences, 0.  A NaN or +inf makes s NaN for good.
 struct Online {
     float m, ref, s;
     static __device__ __forceinline__ Online none() { return Online{neg_inf(), 0.f, 0.f}; }
-    __device__ __forceinline__ void raise(float x, float c) {
-        s = m == neg_inf() ? 0.f : s * ex2((ref - x) * c);
-        m = ref = x;
-    }
-    // `most` is the largest of x[], or NaN if one is.  Masked elements are -inf.
-    template <int N> __device__ __forceinline__ void add(const float (&x)[N], float most, float c) {
-        if (!(most <= m)) raise(most, c);
+    template <int N> __device__ __forceinline__ float sum(const float (&x)[N], float c) const {
         const unsigned long long r2 = f2_pack(-ref, -ref), c2 = f2_pack(c, c);
-        float t0 = 0.f, t1 = 0.f;
+        unsigned long long t = 0;  // two sums
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
             float a, b;
             f2_unpack(f2_mul(f2_add(f2_pack(x[i], x[i + 1]), r2), c2), a, b);
-            t0 += ex2(a);
-            t1 += ex2(b);
+            const unsigned long long e = f2_pack(ex2(a), ex2(b));
+            t = i ? f2_add(t, e) : e;
         }
-        s += t0 + t1;
+        float a, b;
+        f2_unpack(t, a, b);
+        return a + b;
+    }
+    // Masked elements are -inf.  The largest of x[] is looked for only where their sum says that m is too low.
+    template <int N> __device__ __forceinline__ void add(const float (&x)[N], float c) {
+        float t = sum(x, c);
+        if (!(t < 256.f) || s == 0.f) {
+            const float most = largest(x);
+            if (!(most <= m)) {
+                s = s == 0.f ? 0.f : s * ex2((ref - most) * c);
+                m = ref = most;
+                t = sum(x, c);
+            }
+        }
+        s += t;
     }
     __device__ __forceinline__ void merge(const Online& o, float c) {
         if (o.s == 0.f) return;
@@ -107,38 +158,26 @@ struct Online {
     }
 };
 
-__device__ __forceinline__ Online warp_merge(Online o, float c) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        Online p;
-        p.m = __shfl_xor_sync(~0u, o.m, d);
-        p.ref = __shfl_xor_sync(~0u, o.ref, d);
-        p.s = __shfl_xor_sync(~0u, o.s, d);
-        o.merge(p, c);
-    }
-    return o;
-}
-
-// Over the block; every thread gets the result.  `room`: one Online for each warp.
-template <int WARPS> __device__ __forceinline__ Online block_merge(Online o, float c, Online* room) {
-    o = warp_merge(o, c);
-    if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = o;
-    __syncthreads();
-    Online all = Online::none();
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) all.merge(room[w], c);
-    return all;
-}
-
-__device__ __forceinline__ float warp_max_nan(float v) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, d));
-    return v;
-}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
     return v;
+}
+// Over the warp; every lane gets the result.
+__device__ __forceinline__ Online warp_merge(const Online& o, float c) {
+    Online all;
+    all.m = warp_max_nan(o.m);
+    all.ref = all.m == neg_inf() ? 0.f : all.m;
+    all.s = warp_sum(o.s == 0.f ? 0.f : o.s * ex2((o.ref - all.ref) * c));
+    return all;
+}
+// Over the block; every thread gets the result.  `room`: one Online for each warp.
+template <int WARPS> __device__ __forceinline__ Online block_merge(const Online& o, float c, Online* room) {
+    const Online w = warp_merge(o, c);
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) room[threadIdx.x >> 5] = w;
+    __syncthreads();
+    return warp_merge(lane < WARPS ? room[lane] : Online::none(), c);
 }
 
 }  // namespace ddf

@@ -5,17 +5,19 @@
 //   rest[n] = log sum over the classes j that are not among them of exp(x[n,j] / T)
 //
 // What bounds it: the row is read once from memory; everything after that works on its copy in shared memory
-// (rows up to kTopResident bytes) or reads it again out of L2.  One block per row.
-//   1. Every thread takes the largest of its share.  The k-th largest of these NT maxima bounds the row's
-//      k-th largest from below (k of the row's elements reach it), and is close: with m elements a thread
-//      about k + k^2 / (2 NT) elements lie at or above it.  A binary search over the upper 16 bits of the ordered
-//      keys finds it in 16 barriers that count.
+// (rows up to kResidentBytes, brought by bulk copies) or reads it again out of L2.  One block per row.
+//   1. Every thread takes the largest of its share (2-byte types: two at a time).  The k-th largest of these maxima, or,
+//      where that leaves 2 k of them, of the maxima of four threads each, bounds the row's k-th largest from below
+//      (k of the row's elements reach it), and is close: with m elements to a maximum and n maxima some
+//      k + k^2 / (2 n) elements lie at or above it.  One warp finds it by a binary search over the upper 16 bits of the
+//      ordered keys.
 //   2. Elements at or above it go to a list; the others into the running softmax sum.
 //   3. Each listed element counts the elements ahead of it, by one 64-bit key (value, then lower class first):
 //      its place, or, past k, one more summand of the rest.
 // A list that runs over (rows of few distinct values, masked rows) takes the general way instead: a
 // radix selection of the k-th key over four histograms, then one ordered pass that fills in its equals.
 #include <atomic>
+#include <type_traits>
 
 #include "logits.cuh"
 
@@ -25,7 +27,6 @@ extern std::atomic<unsigned long long> g_launches;
 int device_facts(int* sm_count, int** fault, int* index);
 
 constexpr int kTopList = 1024;               // elements at or above the bound that are ranked directly
-constexpr int kTopResident = 72 * 1024;      // three blocks an SM keep their rows in shared memory
 
 // Order of the elements as an unsigned integer: -0 as +0, NaN on top.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -37,6 +38,28 @@ __device__ __forceinline__ float unordered(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
+// The larger elements of two words, NaN where one is.
+template <typename T> __device__ __forceinline__ uint32_t max_words(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) {
+        return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+    } else if constexpr (std::is_same_v<T, __half>) {
+        uint32_t r;
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    } else {
+        uint32_t r;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+}
+template <typename T> __device__ __forceinline__ uint32_t max_granule(const uint4& g) {
+    return max_words<T>(max_words<T>(g.x, g.y), max_words<T>(g.z, g.w));
+}
+template <typename T> __device__ __forceinline__ float max_of_word(uint32_t w) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else return max_nan(Word<T>::get(w, 0), Word<T>::get(w, 1));
+}
+
 struct TopPlan {
     const void* logits;
     void* values;
@@ -45,12 +68,15 @@ struct TopPlan {
     long long stride;
     int V, k;
     float c, T;
+    int* fault;
 };
 
 template <int NT> struct TopShared {
-    unsigned long long list[kTopList];
+    Arrival arrival;
+    float bound;
+
+    unsigned long long list[kTopList];  // before that the maxima, and the general way's histogram
     Online room[NT / 32];
-    int histogram[256];
     int count, above, pick, warp_ties[NT / 32];
 };
 
@@ -61,56 +87,110 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
     extern __shared__ __align__(16) unsigned char copy_raw[];
     uint4* copy = reinterpret_cast<uint4*>(copy_raw);
     __shared__ TopShared<NT> sh;
+    uint32_t* const maxima = reinterpret_cast<uint32_t*>(sh.list);
+    int* const histogram = reinterpret_cast<int*>(sh.list);
+    static_assert(NT * 4 <= sizeof(sh.list) && 1024 <= sizeof(sh.list), "they fit");
     const int tid = threadIdx.x;
     const long long row = blockIdx.x;
     const T* x = reinterpret_cast<const T*>(p.logits) + row * p.stride;
     const Run<T> run(x, p.V);
     const int last = run.granules - 1;
-    auto decode = [&](const uint4& raw, int g, float (&v)[N]) {
-        Granule<T>::get(raw, v);
+    // a granule with -inf for what lies outside the row
+    auto inside = [&](uint4 raw, int g) {
         if (g == 0 || g == last) {
+            float v[N];
+            Granule<T>::get(raw, v);
             const uint32_t out = run.outside(g);
 #pragma unroll
             for (int i = 0; i < N; ++i)
                 if (out >> i & 1u) v[i] = neg_inf();
+            raw = Granule<T>::put(v);
         }
+        return raw;
     };
+    auto granule = [&](int g) { return inside(RESIDENT ? copy[g] : run.load(g), g); };
 
-    if (tid == 0) sh.count = 0;
-    float most = neg_inf();
-    for (int g0 = tid; g0 < run.granules; g0 += NT * UNROLL) {
-        uint4 raw[UNROLL];
+    bool late = false;
+    if (tid == 0) {
+        if constexpr (RESIDENT) fetch_run(run, copy, sh.arrival);
+        sh.count = 0;
+    }
+    uint32_t high_word = Word<T>::put(neg_inf(), neg_inf());
+    if constexpr (RESIDENT) {
+        __syncthreads();
+        for (int c = 0; c * kChunk < run.granules; ++c) {
+            if (!late) late = !await_chunk(sh.arrival, c);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-            if (g0 + u * NT < run.granules) raw[u] = run.load(g0 + u * NT);
+            for (int u = 0; u < kChunk / NT; ++u) {
+                const int g = c * kChunk + u * NT + tid;
+                if (g >= run.granules) break;
+                high_word = max_words<T>(high_word, max_granule<T>(granule(g)));
+            }
+        }
+    } else {
+        for (int g0 = tid; g0 < run.granules; g0 += NT * UNROLL) {
+            uint4 raw[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int g = g0 + u * NT;
-            if (g >= run.granules) break;
-            if constexpr (RESIDENT) copy[g] = raw[u];
-            float v[N];
-            decode(raw[u], g, v);
+            for (int u = 0; u < UNROLL; ++u) raw[u] = run.load(min(g0 + u * NT, last));
 #pragma unroll
-            for (int i = 0; i < N; ++i) most = max_nan(most, v[i]);
+            for (int u = 0; u < UNROLL; ++u)  // (an element in two threads' maxima would count twice)
+                if (g0 + u * NT <= last) high_word = max_words<T>(high_word, max_granule<T>(inside(raw[u], g0 + u * NT)));
         }
     }
-    uint32_t bound = 0;
-    const uint32_t mine = ordered(most) >> 16;
+    {
+        float most = max_of_word<T>(high_word);
+        const bool fours = NT / 4 >= 2 * p.k;
+        if (fours) {
+            most = max_nan(most, __shfl_xor_sync(~0u, most, 1));
+            most = max_nan(most, __shfl_xor_sync(~0u, most, 2));
+        }
+        if (!fours) maxima[tid] = ordered(most) >> 16;
+        else if ((tid & 3) == 0) maxima[tid >> 2] = ordered(most) >> 16;
+        __syncthreads();
+        if (tid < 32) {
+            uint32_t mine[NT / 32];
+            const int n = fours ? NT / 4 : NT;
+#pragma unroll
+            for (int i = 0; i < NT / 32; ++i) mine[i] = i * 32 < n ? maxima[i * 32 + tid] : 0u;
+            uint32_t high = 0, low = 0xffffu;
+#pragma unroll
+            for (int i = 0; i < NT / 32; ++i)
+                if (i * 32 < n) {
+                    high = max(high, mine[i]);
+                    low = min(low, mine[i]);
+                }
+            high = __reduce_max_sync(~0u, high);
+            low = __reduce_min_sync(~0u, low);
+            // the bits that all maxima share are the bound's
+            uint32_t bound = low, bit = high == low ? 0u : 1u << (31 - __clz(high ^ low));
+            if (bit) bound = low & ~(2u * bit - 1u);
 #pragma unroll 1
-    for (uint32_t bit = 0x8000u; bit; bit >>= 1)
-        if (__syncthreads_count(mine >= (bound | bit)) >= p.k) bound |= bit;
-    const float floor_value = unordered(bound << 16);  // NaN where the search ends below -inf: every element passes
+            for (; bit; bit >>= 1) {
+                int reach = 0;
+                if (fours) {
+#pragma unroll
+                    for (int i = 0; i < NT / 128; ++i) reach += mine[i] >= (bound | bit);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NT / 32; ++i) reach += mine[i] >= (bound | bit);
+                }
+                reach = __reduce_add_sync(~0u, reach);
+                if (reach >= p.k) bound |= bit;
+                if (reach >= p.k && reach <= p.k + p.k / 8) break;  // close enough
+            }
+            if (tid == 0) sh.bound = unordered(bound << 16);
+        }
+        __syncthreads();
+    }
+    const float floor_value = sh.bound;  // NaN where the search ends below -inf: every element passes
 
     Online rest = Online::none();
     for (int g = tid; g < run.granules; g += NT) {
+        const uint4 raw = granule(g);
         float v[N];
-        decode(RESIDENT ? copy[g] : run.load(g), g, v);
-        float high = v[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) high = max_nan(high, v[i]);
-        if (!(high < floor_value)) {
+        Granule<T>::get(raw, v);
+        if (!(max_of_word<T>(max_granule<T>(raw)) < floor_value)) {
             const uint32_t out = run.outside(g);
-            high = neg_inf();
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 if (!(v[i] < floor_value)) {
@@ -121,25 +201,29 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
                     }
                     v[i] = neg_inf();
                 }
-                high = max_nan(high, v[i]);
             }
         }
-        rest.add(v, high, p.c);
+        rest.add(v, p.c);
     }
     __syncthreads();
     const int listed = sh.count;
     T* values = reinterpret_cast<T*>(p.values) + row * p.k;
     long long* indices = p.indices + row * p.k;
     auto place = [&](int rank, uint32_t element) {
-        values[rank] = x[element];
+        values[rank] = RESIDENT ? reinterpret_cast<const T*>(copy)[element + run.phase] : x[element];
         indices[rank] = (long long)element;
     };
     if (listed <= kTopList) {
-        for (int i = tid; i < listed; i += NT) {
-            const unsigned long long key = sh.list[i];
+        // four threads an element, each with a quarter of the comparisons
+        for (int i0 = 0; i0 < listed; i0 += NT / 4) {
+            const int i = i0 + (tid >> 2);
+            const unsigned long long key = i < listed ? sh.list[i] : 0ull;
             int rank = 0;
 #pragma unroll 4
-            for (int j = 0; j < listed; ++j) rank += sh.list[j] > key;
+            for (int j = tid & 3; j < listed; j += 4) rank += sh.list[j] > key;
+            rank += __shfl_xor_sync(~0u, rank, 1);
+            rank += __shfl_xor_sync(~0u, rank, 2);
+            if ((tid & 3) || i >= listed) continue;
             if (rank < p.k) {
                 place(rank, 0xffffffffu - (uint32_t)key);
             } else {
@@ -158,23 +242,23 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
         uint32_t prefix = 0;
         int need = p.k;  // of the elements whose upper bytes equal the prefix
         for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += NT) sh.histogram[i] = 0;
+            for (int i = tid; i < 256; i += NT) histogram[i] = 0;
             __syncthreads();
             for (int g = tid; g < run.granules; g += NT) {
                 float v[N];
-                decode(RESIDENT ? copy[g] : run.load(g), g, v);
+                Granule<T>::get(granule(g), v);
                 const uint32_t out = run.outside(g);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const uint32_t key = ordered(v[i]);
                     if (!(out >> i & 1u) && (shift == 24 || (key ^ prefix) >> (shift + 8) == 0))
-                        atomicAdd(&sh.histogram[key >> shift & 255u], 1);
+                        atomicAdd(&histogram[key >> shift & 255u], 1);
                 }
             }
             __syncthreads();
             if (tid == 0) {
                 int above = 0, b = 255;
-                for (; b > 0 && above + sh.histogram[b] < need; --b) above += sh.histogram[b];
+                for (; b > 0 && above + histogram[b] < need; --b) above += histogram[b];
                 sh.pick = b;
                 sh.above = above;
             }
@@ -189,18 +273,16 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
         rest = Online::none();
         for (int g = tid; g < run.granules; g += NT) {
             float v[N];
-            decode(RESIDENT ? copy[g] : run.load(g), g, v);
+            Granule<T>::get(granule(g), v);
             const uint32_t out = run.outside(g);
-            float high = neg_inf();
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const uint32_t key = ordered(v[i]);
                 if (key > prefix && !(out >> i & 1u))
                     sh.list[atomicAdd(&sh.count, 1)] = (unsigned long long)key << 32 | (0xffffffffu - (uint32_t)(g * N + i - run.phase));
                 if (key >= prefix) v[i] = neg_inf();
-                high = max_nan(high, v[i]);
             }
-            rest.add(v, high, p.c);
+            rest.add(v, p.c);
         }
         __syncthreads();
         const int above = sh.count;  // k - need
@@ -241,14 +323,15 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
     }
     rest = block_merge<NT / 32>(rest, p.c, sh.room);
     if (p.rest && tid == 0) p.rest[row] = rest.s == 0.f ? neg_inf() : rest.m / p.T + logf(rest.s);
+    if (late) give_up(p.fault);
 }
 
 template <typename T, int NT>
 static int top_launch(const TopPlan& p, long long rows, cudaStream_t st) {
     const size_t bytes = ((size_t)p.V * sizeof(T) + 15) / 16 * 16 + 16;  // a granule more for a row that starts inside one
-    if (bytes <= kTopResident) {
+    if (bytes <= (size_t)kResidentGranules * 16) {
         if (bytes > 36 * 1024) {  // with the static part beyond what a block gets unasked
-            const cudaError_t e = cudaFuncSetAttribute(top_logits_kernel<T, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTopResident);
+            const cudaError_t e = cudaFuncSetAttribute(top_logits_kernel<T, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
             if (e != cudaSuccess) return (int)e;
         }
         top_logits_kernel<T, NT, true><<<(unsigned)rows, NT, bytes, st>>>(p);
@@ -265,6 +348,7 @@ static int top_choose(const TopPlan& p, long long rows, int sm_count, cudaStream
     // k maxima must be there to bound the k-th largest
     if (granules <= 512 && p.k <= 128) return top_launch<T, 128>(p, rows, st);
     if (granules >= 4096 && rows <= sm_count) return top_launch<T, 1024>(p, rows, st);
+    if (granules >= 2048) return top_launch<T, 512>(p, rows, st);
     return top_launch<T, 256>(p, rows, st);
 }
 
@@ -282,7 +366,7 @@ extern "C" int ddf_b200_top_logits(const void* logits, void* values, long long* 
     int sm = 0, index = 0, *fault = nullptr;
     const int rc = device_facts(&sm, &fault, &index);
     if (rc) return rc;
-    TopPlan p{logits, values, indices, rest, row_stride, (int)classes, k, (float)(1.4426950408889634 / temperature), (float)temperature};
+    TopPlan p{logits, values, indices, rest, row_stride, (int)classes, k, (float)(1.4426950408889634 / temperature), (float)temperature, fault};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (dtype) {
         case DDF_B200_F32: return top_choose<float>(p, rows, sm, st);
