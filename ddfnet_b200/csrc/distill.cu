@@ -19,8 +19,6 @@
 // take a block, or a cluster of blocks whose slices fit shared memory (distill_block_kernel): loss and gradient
 // together then read the row once; across the cluster goes one (maximum, sum) pair a block.
 // A bitmap of the listed classes leaves them out of the running sum; their own values are gathered.
-#include <cooperative_groups.h>
-
 #include <atomic>
 
 #include "logits.cuh"
@@ -352,10 +350,11 @@ __device__ __forceinline__ void send_to_block(uint32_t at, uint32_t bar, uint32_
 
 // RESIDENT: the slice lies in shared memory, brought there by bulk copies that start before anything else and arrive
 // while the entries are read.  Otherwise (classes that fit no cluster's shared memory) it is read from memory by each pass.
-constexpr int kRowThreads = 512;
+constexpr int kRowThreads = 256;
+constexpr int kSliceBytes = 32 * 1024;  // six blocks an SM; up to kResidentBytes where a cluster of eight has to hold more
 
 template <typename T, int MODE, bool RESIDENT>
-__global__ void __launch_bounds__(kRowThreads, 3) distill_block_kernel(const __grid_constant__ DistillPlan p) {
+__global__ void __launch_bounds__(kRowThreads, 6) distill_block_kernel(const __grid_constant__ DistillPlan p) {
     constexpr int N = Granule<T>::N;
     constexpr int NT = kRowThreads;
     static_assert(NT >= kMaxTop && kChunk % NT == 0, "a thread for each entry; a chunk is whole turns of the block");
@@ -387,8 +386,10 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_block_kernel(const __g
         if constexpr (RESIDENT) fetch_run(run, copy, arrival);
         else mbar_fence_init();
     }
+    __syncwarp();
     if constexpr ((MODE & kLoss) != 0) {
-        if (p.slices > 1) cooperative_groups::this_cluster().barrier_arrive();
+        // (the barrier's initialisation is all that the others have to see: its fence is the only one needed)
+        if (p.slices > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
         for (int i = tid; i < (run.granules * N + 31) / 32; i += NT) bits[i] = 0;
     }
     int mine = -1;
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) distill_block_kernel(const __g
         }
         const Online w = warp_merge(others, p.c);
         if ((tid & 31) == 0) room[tid >> 5] = w;
-        if (p.slices > 1) cooperative_groups::this_cluster().barrier_wait();  // every block of the cluster has its barrier
+        if (p.slices > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every block of the cluster has its barrier
         __syncthreads();
         if (tid < 32) {
             others = warp_merge(tid < NT / 32 ? room[tid] : Online::none(), p.c);
@@ -594,11 +595,11 @@ static int distill_launch(DistillPlan p, int sm_count, cudaStream_t st) {
         long long slices = 1;
         if (MODE == kGrad) {
             // blocks on their own, down to 4 KB each where there are few rows
-            slices = (row_bytes + 64 + kResidentBytes - 1) / kResidentBytes;
+            slices = (row_bytes + 64 + kSliceBytes - 1) / kSliceBytes;
             while (p.rows * slices < 2 * sm_count && row_bytes / slices > 4096) slices *= 2;
         } else {
             // a cluster for each row: slices that fit shared memory, or, with few rows, more of them
-            while (slices < 8 && (row_bytes / slices + 64 > kResidentBytes || (p.rows * slices < 2 * sm_count && row_bytes / slices > 8192))) slices *= 2;
+            while (slices < 8 && (row_bytes / slices + 64 > kSliceBytes || (p.rows * slices < 2 * sm_count && row_bytes / slices > 8192))) slices *= 2;
         }
         long long per = (p.V + slices - 1) / slices;
         per = (per + 7) / 8 * 8;  // granules of the slices keep the row's phase

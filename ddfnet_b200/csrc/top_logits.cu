@@ -108,6 +108,11 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
         }
         return raw;
     };
+    // element e of the granules, in the low bits
+    auto lds_elem = [&](uint32_t e) -> uint32_t {
+        if constexpr (sizeof(T) == 4) return reinterpret_cast<const uint32_t*>(copy)[e];
+        else return reinterpret_cast<const uint16_t*>(copy)[e];
+    };
     auto granule = [&](int g) { return inside(RESIDENT ? copy[g] : run.load(g), g); };
 
     bool late = false;
@@ -190,16 +195,20 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
         float v[N];
         Granule<T>::get(raw, v);
         if (!(max_of_word<T>(max_granule<T>(raw)) < floor_value)) {
-            const uint32_t out = run.outside(g);
+            uint32_t hits = 0;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
+            for (int i = 0; i < N; ++i)
                 if (!(v[i] < floor_value)) {
-                    if (!(out >> i & 1u)) {
-                        const int at = atomicAdd(&sh.count, 1);
-                        if (at < kTopList)
-                            sh.list[at] = (unsigned long long)ordered(v[i]) << 32 | (0xffffffffu - (uint32_t)(g * N + i - run.phase));
-                    }
+                    hits |= 1u << i;
                     v[i] = neg_inf();
+                }
+            // (mostly one: element by element, its value from memory, not from a register that the bit would have to select)
+            for (hits &= ~run.outside(g); hits; hits &= hits - 1) {
+                const uint32_t e = (uint32_t)(g * N + __ffs(hits) - 1);
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < kTopList) {
+                    const float value = RESIDENT ? Word<T>::get(lds_elem(e), 0) : Elem<T>::load(x + (int)e - run.phase);
+                    sh.list[at] = (unsigned long long)ordered(value) << 32 | (0xffffffffu - (e - (uint32_t)run.phase));
                 }
             }
         }
@@ -215,7 +224,7 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
     };
     if (listed <= kTopList) {
         // four threads an element, each with a quarter of the comparisons
-        for (int i0 = 0; i0 < listed; i0 += NT / 4) {
+        for (int i0 = 0; i0 + (tid >> 5) * 8 < listed; i0 += NT / 4) {  // (eight elements a warp)
             const int i = i0 + (tid >> 2);
             const unsigned long long key = i < listed ? sh.list[i] : 0ull;
             int rank = 0;
