@@ -484,6 +484,7 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_block_kernel(const __g
         const bool even = (reinterpret_cast<unsigned long long>(out + v0) & 15ull) == (reinterpret_cast<unsigned long long>(x + v0) & 15ull);
         const Others o = shared_others;
         const bool counted = shared_row.counted();
+        char* const out_base = reinterpret_cast<char*>(out + v0 - run.phase);  // of granule 0, where `even`
         for (int c = 0; c * kChunk < run.granules; ++c) {
             if (RESIDENT && MODE == kGrad && !late) late = !await_chunk(arrival, c);
 #pragma unroll
@@ -497,7 +498,12 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_block_kernel(const __g
 #pragma unroll
                     for (int e = 0; e < N; ++e) v[e] = 0.f;
                 }
-                store_granule(run, out + v0, g, even, v);
+                if (even && g > 0 && g + 1 < run.granules) {
+                    const uint4 q = Granule<T>::put(v);
+                    asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(out_base + (long long)g * 16), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
+                } else {
+                    store_granule(run, out + v0, g, even, v);
+                }
             }
         }
         __syncthreads();  // the listed classes' gradients go over what the loop has put there

@@ -11,7 +11,9 @@
 //      (k of the row's elements reach it), and is close: with m elements to a maximum and n maxima some
 //      k + k^2 / (2 n) elements lie at or above it.  One warp finds it by a binary search over the upper 16 bits of the
 //      ordered keys.
-//   2. Elements at or above it go to a list; the others into the running softmax sum.
+//   2. Granules without an element at or above it go into the running softmax sum, the others to a list: a hundred
+//      of them a row, in every second warp's turn, would cost as much as all the rest if they were taken apart there.
+//      Their elements then get a thread each, and go to the sum or to the list of elements.
 //   3. Each listed element counts the elements ahead of it, by one 64-bit key (value, then lower class first):
 //      its place, or, past k, one more summand of the rest.
 // A list that runs over (rows of few distinct values, masked rows) takes the general way instead: a
@@ -26,7 +28,8 @@ namespace ddf {
 extern std::atomic<unsigned long long> g_launches;
 int device_facts(int* sm_count, int** fault, int* index);
 
-constexpr int kTopList = 1024;               // elements at or above the bound that are ranked directly
+constexpr int kTopList = 512;                // elements at or above the bound that are ranked directly
+constexpr int kTopGranules = 512;            // granules that have one
 
 // Order of the elements as an unsigned integer: -0 as +0, NaN on top.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -60,6 +63,19 @@ template <typename T> __device__ __forceinline__ float max_of_word(uint32_t w) {
     else return max_nan(Word<T>::get(w, 0), Word<T>::get(w, 1));
 }
 
+// Which elements of a word do not lie below `bound`'s (NaN does not): all bits of each.
+template <typename T> __device__ __forceinline__ uint32_t not_below(uint32_t w, uint32_t bound) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w) < __uint_as_float(bound) ? 0u : ~0u;
+    else if constexpr (std::is_same_v<T, __half>) return __hgeu2_mask(*reinterpret_cast<__half2*>(&w), *reinterpret_cast<__half2*>(&bound));
+    else return __hgeu2_mask(*reinterpret_cast<__nv_bfloat162*>(&w), *reinterpret_cast<__nv_bfloat162*>(&bound));
+}
+// The bound as a word of elements, rounded down.
+template <typename T> __device__ __forceinline__ uint32_t bound_word(float b) {
+    if constexpr (sizeof(T) == 4) return __float_as_uint(b);
+    else if constexpr (std::is_same_v<T, __half>) return (uint32_t)__half_as_ushort(__float2half_rd(b)) * 0x10001u;
+    else return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rd(b)) * 0x10001u;
+}
+
 struct TopPlan {
     const void* logits;
     void* values;
@@ -73,11 +89,12 @@ struct TopPlan {
 
 template <int NT> struct TopShared {
     Arrival arrival;
-    float bound;
+    uint32_t bound;
 
     unsigned long long list[kTopList];  // before that the maxima, and the general way's histogram
     Online room[NT / 32];
-    int count, above, pick, warp_ties[NT / 32];
+    int granules[kTopGranules];
+    int hits, count, above, pick, warp_ties[NT / 32];
 };
 
 template <typename T, int NT, bool RESIDENT>
@@ -109,16 +126,16 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
         return raw;
     };
     // element e of the granules, in the low bits
-    auto lds_elem = [&](uint32_t e) -> uint32_t {
+    auto element_word = [&](int e) -> uint32_t {
         if constexpr (sizeof(T) == 4) return reinterpret_cast<const uint32_t*>(copy)[e];
         else return reinterpret_cast<const uint16_t*>(copy)[e];
     };
-    auto granule = [&](int g) { return inside(RESIDENT ? copy[g] : run.load(g), g); };
+    auto granule = [&](int g) { return RESIDENT ? copy[g] : inside(run.load(g), g); };
 
     bool late = false;
     if (tid == 0) {
         if constexpr (RESIDENT) fetch_run(run, copy, sh.arrival);
-        sh.count = 0;
+        sh.count = sh.hits = 0;
     }
     uint32_t high_word = Word<T>::put(neg_inf(), neg_inf());
     if constexpr (RESIDENT) {
@@ -127,9 +144,11 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
             if (!late) late = !await_chunk(sh.arrival, c);
 #pragma unroll
             for (int u = 0; u < kChunk / NT; ++u) {
-                const int g = c * kChunk + u * NT + tid;
+                const int g = c * kChunk + u * NT + tid;  // (pass 2 gives the same thread the same granules)
                 if (g >= run.granules) break;
-                high_word = max_words<T>(high_word, max_granule<T>(granule(g)));
+                uint4 raw = copy[g];
+                if (g == 0 || g == last) copy[g] = raw = inside(raw, g);
+                high_word = max_words<T>(high_word, max_granule<T>(raw));
             }
         }
     } else {
@@ -183,39 +202,46 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
                 if (reach >= p.k) bound |= bit;
                 if (reach >= p.k && reach <= p.k + p.k / 8) break;  // close enough
             }
-            if (tid == 0) sh.bound = unordered(bound << 16);
+            if (tid == 0) sh.bound = bound_word<T>(unordered(bound << 16));
         }
         __syncthreads();
     }
-    const float floor_value = sh.bound;  // NaN where the search ends below -inf: every element passes
+    const uint32_t bound = sh.bound;  // NaN where the search ends below -inf: every element passes
+    const float floor_of_word = Word<T>::get(bound, 0);
 
+    // granules without such an element go into the sum, the others to a list
     Online rest = Online::none();
+#pragma unroll 2
     for (int g = tid; g < run.granules; g += NT) {
         const uint4 raw = granule(g);
+        if (not_below<T>(max_granule<T>(raw), bound)) {
+            const int at = atomicAdd(&sh.hits, 1);
+            if (at < kTopGranules) sh.granules[at] = g;
+            continue;
+        }
         float v[N];
         Granule<T>::get(raw, v);
-        if (!(max_of_word<T>(max_granule<T>(raw)) < floor_value)) {
-            uint32_t hits = 0;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (!(v[i] < floor_value)) {
-                    hits |= 1u << i;
-                    v[i] = neg_inf();
-                }
-            // (mostly one: element by element, its value from memory, not from a register that the bit would have to select)
-            for (hits &= ~run.outside(g); hits; hits &= hits - 1) {
-                const uint32_t e = (uint32_t)(g * N + __ffs(hits) - 1);
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < kTopList) {
-                    const float value = RESIDENT ? Word<T>::get(lds_elem(e), 0) : Elem<T>::load(x + (int)e - run.phase);
-                    sh.list[at] = (unsigned long long)ordered(value) << 32 | (0xffffffffu - (e - (uint32_t)run.phase));
-                }
-            }
-        }
         rest.add(v, p.c);
     }
     __syncthreads();
-    const int listed = sh.count;
+    // ... whose elements are looked at by a thread each
+    const int hits = sh.hits;
+    if (hits <= kTopGranules) {
+        for (int i = tid; i < hits * N; i += NT) {
+            const int g = sh.granules[i / N], e = g * N + i % N - run.phase;
+            if (e < 0 || e >= p.V) continue;
+            const float v = RESIDENT ? Word<T>::get(element_word(e + run.phase), 0) : Elem<T>::load(x + e);
+            if (!(v < floor_of_word)) {
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < kTopList) sh.list[at] = (unsigned long long)ordered(v) << 32 | (0xffffffffu - (uint32_t)e);
+            } else {
+                const float one[2] = {v, neg_inf()};
+                rest.add(one, p.c);
+            }
+        }
+    }
+    __syncthreads();
+    const int listed = hits <= kTopGranules ? sh.count : kTopList + 1;
     T* values = reinterpret_cast<T*>(p.values) + row * p.k;
     long long* indices = p.indices + row * p.k;
     auto place = [&](int rank, uint32_t element) {
