@@ -52,7 +52,7 @@ SYMBOLS = (
     "ddf_b200_sfnorm", "ddf_b200_sfnorm_backward", "ddf_b200_maxpool_nhwc",
     "ddf_b200_top_logits", "ddf_b200_distill_forward", "ddf_b200_distill_backward", "ddf_b200_distill_loss_grad",
     "ddf_b200_linear_workspace", "ddf_b200_linear_forward", "ddf_b200_linear_backward_workspace",
-    "ddf_b200_linear_backward",
+    "ddf_b200_linear_backward", "ddf_b200_linear_waitlimit",
     "ddf_b200_noop", "ddf_b200_rate_probe_bytes", "ddf_b200_rate_probe",
 )
 
@@ -109,6 +109,8 @@ def load() -> ctypes.CDLL:
         L.ddf_b200_linear_workspace.argtypes = [linear]
         L.ddf_b200_linear_forward.restype = i
         L.ddf_b200_linear_forward.argtypes = [linear, vp, vp, vp, sz, vp]
+        L.ddf_b200_linear_waitlimit.restype = i
+        L.ddf_b200_linear_waitlimit.argtypes = [linear, vp, vp, sz, ll, i, vp]
         L.ddf_b200_linear_backward_workspace.restype = sz
         L.ddf_b200_linear_backward_workspace.argtypes = [linear, vp, ll] + [vp] * 4
         L.ddf_b200_linear_backward.restype = i

@@ -298,9 +298,15 @@ template <typename T, bool AT, bool BT> static auto kernel_of(int bn, int act) {
     return bn == 256 ? linear_kernel<T, 256, AT, BT, kActNone> : bn == 128 ? linear_kernel<T, 128, AT, BT, kActNone> : linear_kernel<T, 64, AT, BT, kActNone>;
 }
 
+// Of a product's waits: their limit, and whether they are made to run out.
+struct Wait {
+    long long limit = kWaitCycles;
+    bool starve = false, test = false;
+};
+
 // D (M x N) = A B^T.  at / bt: the matrix given is stored with the reduction as its rows.
 template <typename T, bool AT, bool BT>
-static int product(const Matrix& a, const Matrix& b, long long M, long long N, long long K, const Epilogue& out, float* partial, int dtype, long long limit,
+static int product(const Matrix& a, const Matrix& b, long long M, long long N, long long K, const Epilogue& out, float* partial, int dtype, Wait wait,
                    cudaStream_t st) {
     int sm = 0, index = 0, *fault = nullptr;
     int rc = device_facts(&sm, &fault, &index);
@@ -338,7 +344,8 @@ static int product(const Matrix& a, const Matrix& b, long long M, long long N, l
     const uint32_t type = dtype == DDF_B200_BF16 ? 1u : 0u;
     p.idesc = 1u << 4 | type << 7 | type << 10 | (AT ? 1u << 15 : 0u) | (BT ? 1u << 16 : 0u) | (uint32_t)(cut.bn / 8) << 17 | (uint32_t)(kTileM / 16) << 24;
     p.fault = fault;
-    p.limit = limit;
+    p.limit = wait.limit;
+    p.starve = wait.starve ? 16u : 0u;
     const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
     if (items > 0x7fffffffll) return DDF_B200_E_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
@@ -427,11 +434,11 @@ static int check_linear(const ddf_b200_linear_args* q) {
 static bool by_four(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0 && ld % 4 == 0; }
 
 template <typename T>
-static int forward(const ddf_b200_linear_args* q, void* y, void* aux, Space& ws, size_t have, long long limit, cudaStream_t st, bool only_size, int sm) {
+static int forward(const ddf_b200_linear_args* q, void* y, void* aux, Space& ws, size_t have, Wait wait, cudaStream_t st, bool only_size, int sm) {
     const long long M = q->rows, N = q->outputs, K = q->inputs;
     Epilogue e{y, aux, q->bias, q->residual, N, q->residual_stride, q->activation, q->after, 0};
     e.vec = by_four(y, N) && (!aux || by_four(aux, N)) && (!q->residual || by_four(q->residual, q->residual_stride));
-    if (M <= kFewRows && limit == kWaitCycles) {
+    if (M <= kFewRows && !wait.test) {
         if (only_size) return 0;
         if (M == 1) return rows_launch<T, 1, 1>(q, e, st);
         if (M == 2) return rows_launch<T, 2, 1>(q, e, st);
@@ -445,7 +452,7 @@ static int forward(const ddf_b200_linear_args* q, void* y, void* aux, Space& ws,
     if (ws.used > have) return DDF_B200_E_WORKSPACE;
     const int rc = pack<T>(x, xp, w, wp, st);
     if (rc) return rc;
-    return product<T, false, false>(x, w, M, N, K, e, partial, q->dtype, limit, st);
+    return product<T, false, false>(x, w, M, N, K, e, partial, q->dtype, wait, st);
 }
 
 template <typename T>
@@ -497,11 +504,11 @@ static int backward(const ddf_b200_linear_args* q, const void* gy, long long gy_
     Epilogue e{};
     if (gx) {
         e.y = gx; e.ldy = K; e.vec = by_four(gx, K);
-        if ((rc = product<T, false, true>(gz, w, M, K, N, e, partial, q->dtype, kWaitCycles, st))) return rc;
+        if ((rc = product<T, false, true>(gz, w, M, K, N, e, partial, q->dtype, Wait(), st))) return rc;
     }
     if (gw) {
         e.y = gw; e.ldy = K; e.vec = by_four(gw, K);
-        if ((rc = product<T, true, true>(gz, x, N, K, M, e, partial, q->dtype, kWaitCycles, st))) return rc;
+        if ((rc = product<T, true, true>(gz, x, N, K, M, e, partial, q->dtype, Wait(), st))) return rc;
     }
     return 0;
 }
@@ -515,7 +522,7 @@ size_t ddf_b200_linear_workspace(const ddf_b200_linear_args* q) {
     int sm = 0, index = 0, *fault = nullptr;
     if (check_linear(q) || device_facts(&sm, &fault, &index)) return 0;
     Space ws{nullptr};
-    forward<__half>(q, nullptr, nullptr, ws, 0, kWaitCycles, nullptr, true, sm);
+    forward<__half>(q, nullptr, nullptr, ws, 0, Wait(), nullptr, true, sm);
     return ws.used;
 }
 
@@ -528,8 +535,26 @@ int ddf_b200_linear_forward(const ddf_b200_linear_args* q, void* y, void* aux, v
     if ((rc = device_facts(&sm, &fault, &index))) return rc;
     Space ws{(char*)workspace};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    return q->dtype == DDF_B200_F16 ? forward<__half>(q, y, aux, ws, workspace_bytes, kWaitCycles, st, false, sm)
-                                    : forward<__nv_bfloat16>(q, y, aux, ws, workspace_bytes, kWaitCycles, st, false, sm);
+    return q->dtype == DDF_B200_F16 ? forward<__half>(q, y, aux, ws, workspace_bytes, Wait(), st, false, sm)
+                                    : forward<__nv_bfloat16>(q, y, aux, ws, workspace_bytes, Wait(), st, false, sm);
+}
+
+int ddf_b200_linear_waitlimit(const ddf_b200_linear_args* q, void* y, void* workspace, size_t workspace_bytes, long long wait_cycles, int starve, void* stream) {
+    using namespace ddf;
+    int rc = check_linear(q);
+    if (rc) return rc;
+    if (!y || (workspace_bytes && !workspace)) return DDF_B200_E_NULL;
+    if (wait_cycles < 1) return DDF_B200_E_ARGUMENT;
+    int sm = 0, index = 0, *fault = nullptr;
+    if ((rc = device_facts(&sm, &fault, &index))) return rc;
+    Space ws{(char*)workspace};
+    Wait wait;
+    wait.limit = wait_cycles;
+    wait.starve = starve != 0;
+    wait.test = true;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return q->dtype == DDF_B200_F16 ? forward<__half>(q, y, nullptr, ws, workspace_bytes, wait, st, false, sm)
+                                    : forward<__nv_bfloat16>(q, y, nullptr, ws, workspace_bytes, wait, st, false, sm);
 }
 
 size_t ddf_b200_linear_backward_workspace(const ddf_b200_linear_args* q, const void* gy, long long gy_stride, const void* gx, const void* gw, const void* gb,

@@ -153,6 +153,7 @@ struct LinearPlan {
     uint32_t idesc;
     int* fault;
     long long limit;        // of a wait, in clocks
+    uint32_t starve;        // bytes announced that never come (self-test)
 };
 
 // Work item -> tile and split: tiles of eight blocks of rows side by side, so that the tiles in flight share operands.
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
                 if (__any_sync(~0u, !mbar_wait_for(empty(stage), phase ^ 1u, p.limit))) { late = true; break; }
                 const uint32_t to = base + (uint32_t)stage * kStage;
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(full(stage), kStage);
+                    mbar_arrive_expect_tx(full(stage), kStage + p.starve);
                     if constexpr (AT) {
 #pragma unroll
                         for (int i = 0; i < kTileM / 64; ++i)

@@ -29,7 +29,7 @@ extern std::atomic<unsigned long long> g_launches;
 int device_facts(int* sm_count, int** fault, int* index);
 
 constexpr int kTopList = 512;                // elements at or above the bound that are ranked directly
-constexpr int kTopGranules = 512;            // granules that have one
+constexpr int kTopGranules = 1024;           // granules that have one, an equal part for each warp
 
 // Order of the elements as an unsigned integer: -0 as +0, NaN on top.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -93,8 +93,8 @@ template <int NT> struct TopShared {
 
     unsigned long long list[kTopList];  // before that the maxima, and the general way's histogram
     Online room[NT / 32];
-    int granules[kTopGranules];
-    int hits, count, above, pick, warp_ties[NT / 32];
+    int granules[kTopGranules];         // after that the listed elements past k, by their ranks
+    int count, above, pick, warp_ties[NT / 32];
 };
 
 template <typename T, int NT, bool RESIDENT>
@@ -106,6 +106,8 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
     __shared__ TopShared<NT> sh;
     uint32_t* const maxima = reinterpret_cast<uint32_t*>(sh.list);
     int* const histogram = reinterpret_cast<int*>(sh.list);
+    float* const extra = reinterpret_cast<float*>(sh.granules);
+    static_assert(kTopList <= kTopGranules, "they fit");
     static_assert(NT * 4 <= sizeof(sh.list) && 1024 <= sizeof(sh.list), "they fit");
     const int tid = threadIdx.x;
     const long long row = blockIdx.x;
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
     bool late = false;
     if (tid == 0) {
         if constexpr (RESIDENT) fetch_run(run, copy, sh.arrival);
-        sh.count = sh.hits = 0;
+        sh.count = 0;
     }
     uint32_t high_word = Word<T>::put(neg_inf(), neg_inf());
     if constexpr (RESIDENT) {
@@ -209,39 +211,49 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
     const uint32_t bound = sh.bound;  // NaN where the search ends below -inf: every element passes
     const float floor_of_word = Word<T>::get(bound, 0);
 
-    // granules without such an element go into the sum, the others to a list
+    // granules without such an element go into the sum, the others to the warp's list
+    constexpr int kLists = kTopGranules / (NT / 32);
+    const int lane = tid & 31, warp = tid >> 5;
+    int* const list = sh.granules + warp * kLists;
+    int hits = 0;
     Online rest = Online::none();
 #pragma unroll 2
-    for (int g = tid; g < run.granules; g += NT) {
-        const uint4 raw = granule(g);
-        if (not_below<T>(max_granule<T>(raw), bound)) {
-            const int at = atomicAdd(&sh.hits, 1);
-            if (at < kTopGranules) sh.granules[at] = g;
-            continue;
+    for (int g0 = warp * 32; g0 < run.granules; g0 += NT) {
+        const int g = g0 + lane;
+        uint4 raw;
+        bool hit = false;
+        if (g < run.granules) {
+            raw = granule(g);
+            hit = not_below<T>(max_granule<T>(raw), bound) != 0;
         }
-        float v[N];
-        Granule<T>::get(raw, v);
-        rest.add(v, p.c);
-    }
-    __syncthreads();
-    // ... whose elements are looked at by a thread each
-    const int hits = sh.hits;
-    if (hits <= kTopGranules) {
-        for (int i = tid; i < hits * N; i += NT) {
-            const int g = sh.granules[i / N], e = g * N + i % N - run.phase;
-            if (e < 0 || e >= p.V) continue;
-            const float v = RESIDENT ? Word<T>::get(element_word(e + run.phase), 0) : Elem<T>::load(x + e);
-            if (!(v < floor_of_word)) {
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < kTopList) sh.list[at] = (unsigned long long)ordered(v) << 32 | (0xffffffffu - (uint32_t)e);
-            } else {
-                const float one[2] = {v, neg_inf()};
-                rest.add(one, p.c);
-            }
+        const uint32_t votes = __ballot_sync(~0u, hit);
+        if (votes) {
+            const int at = hits + __popc(votes & ((1u << lane) - 1u));
+            if (hit && at < kLists) list[at] = g;
+            hits += __popc(votes);
+        }
+        if (g < run.granules && !hit) {
+            float v[N];
+            Granule<T>::get(raw, v);
+            rest.add(v, p.c);
         }
     }
-    __syncthreads();
-    const int listed = hits <= kTopGranules ? sh.count : kTopList + 1;
+    __syncwarp();
+    // ... whose elements are looked at by a lane each, always the same one: the sum has one order
+    for (int i = lane; i < min(hits, kLists) * N; i += 32) {
+        const int e = list[i / N] * N + i % N - run.phase;
+        if (e < 0 || e >= p.V) continue;
+        const float v = RESIDENT ? Word<T>::get(element_word(e + run.phase), 0) : Elem<T>::load(x + e);
+        if (!(v < floor_of_word)) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kTopList) sh.list[at] = (unsigned long long)ordered(v) << 32 | (0xffffffffu - (uint32_t)e);
+        } else {
+            const float one[2] = {v, neg_inf()};
+            rest.add(one, p.c);
+        }
+    }
+    const bool over = __syncthreads_or(hits > kLists);
+    const int listed = over ? kTopList + 1 : sh.count;
     T* values = reinterpret_cast<T*>(p.values) + row * p.k;
     long long* indices = p.indices + row * p.k;
     auto place = [&](int rank, uint32_t element) {
@@ -262,15 +274,14 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
             if (rank < p.k) {
                 place(rank, 0xffffffffu - (uint32_t)key);
             } else {
-                Online one;
-                one.m = unordered((uint32_t)(key >> 32));
-                if (one.m != neg_inf()) {
-                    if (isinf(one.m)) one.m = __int_as_float(0x7fc00000);  // a sum with +inf has no finite logarithm: as NaN
-                    one.ref = one.m;
-                    one.s = one.m == one.m ? 1.f : one.m;
-                    rest.merge(one, p.c);
-                }
+                extra[rank - p.k] = unordered((uint32_t)(key >> 32));
             }
+        }
+        // (in the order of their ranks, not of their arrival in the list)
+        __syncthreads();
+        for (int i = tid; i < listed - p.k; i += NT) {
+            const float one[2] = {extra[i], neg_inf()};
+            rest.add(one, p.c);
         }
     } else {
         // radix selection: the upper bytes of the k-th largest key, one histogram each
@@ -350,10 +361,8 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopPlan p) {
         }
         const float tie = unordered(prefix);
         if (left && tie != neg_inf()) {
-            Online some;
-            some.m = some.ref = tie;
-            some.s = isinf(tie) || !(tie == tie) ? __int_as_float(0x7fc00000) : (float)left;
-            rest.merge(some, p.c);
+            // +inf and NaN make the sum NaN
+            rest.merge(Online{tie, tie, isinf(tie) || !(tie == tie) ? __int_as_float(0x7fc00000) : (float)left}, p.c);
         }
     }
     rest = block_merge<NT / 32>(rest, p.c, sh.room);

@@ -130,16 +130,19 @@ class DDFResNet(nn.Module):
                 nn.init.ones_(m.weight)
                 nn.init.zeros_(m.bias)
 
-    def forward(self, x):
+    def features(self, x):
+        """The pooled features (B, 2048) that the classifier ``fc`` takes."""
         if self.fused_inference:
             c = self.conv1
             x = self.maxpool(torch.cudnn_convolution_relu(x, c.weight, c.bias, c.stride, c.padding,
                                                           c.dilation, 1))
-            x = self.layer4(self.layer3(self.layer2(self.layer1(x))))
-            return self.fc(torch.flatten(self.global_pool(x), 1))
-        x = self.maxpool(self.act1(self.bn1(self.conv1(x))))
+        else:
+            x = self.maxpool(self.act1(self.bn1(self.conv1(x))))
         x = self.layer4(self.layer3(self.layer2(self.layer1(x))))
-        return self.fc(torch.flatten(self.global_pool(x), 1))
+        return torch.flatten(self.global_pool(x), 1)
+
+    def forward(self, x):
+        return self.fc(self.features(x))
 
     def ddf_layers(self):
         """The DDFPack modules in network order."""

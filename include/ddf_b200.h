@@ -446,6 +446,11 @@ typedef struct ddf_b200_linear_args {
 size_t ddf_b200_linear_workspace(const ddf_b200_linear_args* args);
 int ddf_b200_linear_forward(const ddf_b200_linear_args* args, void* y, void* aux, void* workspace,
                             size_t workspace_bytes, void* stream);
+/* Self-test of the product's bounded waits, as ddf_b200_forward_waitlimit: every wait gives up after `wait_cycles`
+ * clocks; with `starve` != 0 no stage of operands is ever complete.  The kernel then records fault 6 and ends with y
+ * unwritten. */
+int ddf_b200_linear_waitlimit(const ddf_b200_linear_args* args, void* y, void* workspace, size_t workspace_bytes,
+                              long long wait_cycles, int starve, void* stream);
 /*
  * Backward, from the gradient gy (rows gy_stride apart) and aux (ACT_NONE: not read):
  *   gz = gy act'(z);  gx = gz W;  gw = gz^T x;  gb = column sums of gz;  gr = gz
