@@ -181,16 +181,18 @@ __device__ __noinline__ void merge_repeated(int* cls, float* a, float* s, int K,
     sync();
 }
 
-// Factor of the row's gradient: upstream, the loss scale and the mean's count, times T.  Whole warps.
-__device__ __forceinline__ float grad_factor(const DistillPlan& p, long long row) {
+// Factor of the row's gradient: upstream, the loss scale and the mean's count, times T.  Whole warps; `n` is the lane's
+// part of the count.
+__device__ __forceinline__ int count_part(const DistillPlan& p) {
+    int n = 0;
+    if (p.counts)
+        for (int i = threadIdx.x & 31; i < p.n_counts; i += 32) n += __ldg(p.counts + i);
+    return n;
+}
+__device__ __forceinline__ float grad_factor(const DistillPlan& p, long long row, int n) {
     float g = p.scale * p.T;
     if (p.upstream) g *= __ldg(p.upstream + row * p.upstream_stride);
-    if (p.counts) {
-        int n = 0;
-        for (int i = threadIdx.x & 31; i < p.n_counts; i += 32) n += __ldg(p.counts + i);
-        n = __reduce_add_sync(~0u, n);
-        g /= (float)max(n, 1);
-    }
+    if (p.counts) g /= (float)max(__reduce_add_sync(~0u, n), 1);
     return g;
 }
 
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_warp_kernel(const __gr
     if constexpr (MODE & kGrad) {
         T* out = reinterpret_cast<T*>(p.grad) + row * p.V;
         const bool even = (reinterpret_cast<unsigned long long>(out) & 15ull) == (reinterpret_cast<unsigned long long>(x) & 15ull);
-        const float g = grad_factor(p, row);
+        const float g = grad_factor(p, row, count_part(p));
         const Others o = others_of(r, g);
         const bool counted = r.counted();
 #pragma unroll
@@ -365,6 +367,7 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_block_kernel(const __g
     __shared__ Online room[NT / 32];
     __shared__ __align__(16) float4 peers[8];
     __shared__ unsigned long long peers_bar;
+    __shared__ int flags[2];  // some entry is there; a class is listed twice
     __shared__ Arrival arrival;
     __shared__ Row shared_row;
     __shared__ Others shared_others;
@@ -380,62 +383,45 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_block_kernel(const __g
     uint32_t* bits = reinterpret_cast<uint32_t*>(raw_shared + (RESIDENT ? (size_t)run.granules * 16 : 0));
     bool late = false;
 
-    // ---- while the slice arrives: the entries, the teacher's softmax
-    if (tid == 0) {
+    // ---- while the slice arrives: the entries.  What they point at (value, own logit) is needed after the first pass only,
+    // and stays on its way until then.
+    if (tid == NT - 32) {
         if constexpr ((MODE & kLoss) != 0) mbar_init(smem_u32(&peers_bar), 1);
         if constexpr (RESIDENT) fetch_run(run, copy, arrival);
         else mbar_fence_init();
     }
     __syncwarp();
+    // (the barrier's initialisation is all that the cluster's others have to see: its fence is the only one needed)
+    if ((MODE & kLoss) && p.slices > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    int mine = -1;
+    if (tid < K) mine = entry_class(p, row * K + tid);
+    float my_a = neg_inf(), my_s = neg_inf();
+    if (mine >= 0) {
+        my_a = entry_value(p.values, row * K + tid, p.values_dtype) / p.T;
+        my_s = Elem<T>::load(x + mine);
+    }
+    float rest = p.rest ? __ldg(p.rest + row) : neg_inf();
+    const int counted_rows = (MODE & kGrad) && tid < 32 ? count_part(p) : 0;
+    if (tid < K) cls[tid] = mine;
+    if (tid < 32) flags[tid & 1] = 0;
     if constexpr ((MODE & kLoss) != 0) {
-        // (the barrier's initialisation is all that the others have to see: its fence is the only one needed)
-        if (p.slices > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
         for (int i = tid; i < (run.granules * N + 31) / 32; i += NT) bits[i] = 0;
     }
-    int mine = -1;
-    if (tid < K) {
-        mine = entry_class(p, row * K + tid);
-        cls[tid] = mine;
-        a[tid] = mine < 0 ? neg_inf() : entry_value(p.values, row * K + tid, p.values_dtype) / p.T;
-        s[tid] = mine < 0 ? neg_inf() : Elem<T>::load(x + mine);
-    }
-    if constexpr ((MODE & kGrad) != 0) {
-        if (tid >= NT - 32) {
-            const float f = grad_factor(p, row);
-            if (tid == NT - 1) shared_factor = f;
+    __syncthreads();
+    if (mine >= 0) {
+        flags[0] = 1;
+        if ((MODE & kLoss) && mine >= v0 && mine < v0 + run.len) {
+            const uint32_t at = (uint32_t)(mine - v0 + run.phase), bit = 1u << (at & 31u);
+            if (atomicOr(bits + (at >> 5), bit) & bit) flags[1] = 1;  // a class listed twice: both fall into one slice
         }
     }
-    const bool any = __syncthreads_or(mine >= 0);
-    const float rest = any && p.rest ? __ldg(p.rest + row) : neg_inf();
     Row r;
-    bool repeated;
     if constexpr ((MODE & kLoss) != 0) {
-        bool twice = false;
-        if (mine >= 0) {
-            if (mine >= v0 && mine < v0 + run.len) {
-                const uint32_t at = (uint32_t)(mine - v0 + run.phase);
-                atomicOr(bits + (at >> 5), 1u << (at & 31u));
-            }
-            for (int i = 0; i < tid; i += 4) {
-                const int4 c = *reinterpret_cast<const int4*>(cls + i);
-                twice |= c.x == mine || (i + 1 < tid && c.y == mine) || (i + 2 < tid && c.z == mine) || (i + 3 < tid && c.w == mine);
-            }
-        }
         if (tid == NT - 1) atomicOr(bits, run.outside(0));
         if (tid == NT - 2) atomicOr(bits + ((run.granules - 1) * N >> 5), run.outside(run.granules - 1) << ((run.granules - 1) * N & 31));
-        repeated = __syncthreads_or(twice);
-    } else {
-        r = get_stats(p.stats + row * kStats, rest);
-        repeated = r.repeated;
-    }
-    if (repeated) {
-        merge_repeated(cls, a, s, K, tid, NT, [] { __syncthreads(); });
-        if (tid < K) mine = cls[tid];
-    }
+        __syncthreads();
 
-    // ---- the sum over the others; then one warp finds what the whole block needs
-    if constexpr ((MODE & kLoss) != 0) {
-        if (tid < 32) teacher_buckets(r, a, K, rest);
+        // ---- the sum over the others; then one warp finds what the whole block needs
         Online others = Online::none();
         for (int c = 0; c * kChunk < run.granules; ++c) {
             if (RESIDENT && !late) late = !await_chunk(arrival, c);
@@ -452,31 +438,60 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_block_kernel(const __g
         }
         const Online w = warp_merge(others, p.c);
         if ((tid & 31) == 0) room[tid >> 5] = w;
+        if (tid < K) {
+            a[tid] = my_a;
+            s[tid] = my_s;
+        }
         if (p.slices > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every block of the cluster has its barrier
         __syncthreads();
         if (tid < 32) {
             others = warp_merge(tid < NT / 32 ? room[tid] : Online::none(), p.c);
+            bool repeated = flags[1] != 0;
+            if (!flags[0]) rest = neg_inf();
+            const uint32_t bar = smem_u32(&peers_bar);
             if (p.slices > 1) {
                 // to every block of the cluster, with word to the one that waits there: no barrier of all its threads
-                const uint32_t bar = smem_u32(&peers_bar);
                 if (tid == 0) mbar_arrive_expect_tx(bar, (uint32_t)p.slices * 16u);
                 __syncwarp();
-                if (tid < p.slices) send_to_block(smem_u32(&peers[rank]), bar, tid, make_float4(others.m, others.ref, others.s, 0.f));
+                if (tid < p.slices) send_to_block(smem_u32(&peers[rank]), bar, tid, make_float4(others.m, others.ref, others.s, repeated ? 1.f : 0.f));
+            }
+            teacher_buckets(r, a, K, rest);
+            if (p.slices > 1) {
                 if (!late) late = !mbar_wait(bar, 0);
                 __syncwarp();
                 const float4 q = tid < p.slices ? peers[tid] : make_float4(neg_inf(), 0.f, 0.f, 0.f);
                 others = warp_merge(Online{q.x, q.y, q.z}, p.c);
+                repeated = __any_sync(~0u, q.w != 0.f);
+                asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this block has all that was sent to it
+            }
+            if (repeated) {
+                merge_repeated(cls, a, s, K, tid, 32, [] { __syncwarp(); });
+                teacher_buckets(r, a, K, rest);
             }
             student_buckets(r, s, K, others, p.c);
             r.repeated = repeated;
+        } else if (p.slices > 1) {
+            asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+        }
+    } else {
+        if (tid < K) {
+            a[tid] = my_a;
+            s[tid] = my_s;
+        }
+        __syncthreads();
+        if (tid < 32) {
+            r = get_stats(p.stats + row * kStats, flags[0] ? rest : neg_inf());
+            if (r.repeated) merge_repeated(cls, a, s, K, tid, 32, [] { __syncwarp(); });
         }
     }
     if constexpr ((MODE & kGrad) != 0) {
         if (tid < 32) {
-            const Others o = others_of(r, shared_factor);
+            const float f = grad_factor(p, row, counted_rows);
+            const Others o = others_of(r, f);
             if (tid == 0) {
                 shared_row = r;
                 shared_others = o;
+                shared_factor = f;
             }
         }
         __syncthreads();
@@ -507,6 +522,7 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_block_kernel(const __g
             }
         }
         __syncthreads();  // the listed classes' gradients go over what the loop has put there
+        if (tid < K) mine = cls[tid];  // (repeated ones have gone)
         if (counted && mine >= v0 && mine < v0 + run.len) {
             const Row q = shared_row;
             Elem<T>::store(out + mine, shared_factor * q_minus_p(log2_p(q, a[tid]), log2_q(q, s[tid], p.c)));
@@ -523,12 +539,9 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_block_kernel(const __g
     }
     if (late) give_up(p.fault);
     if constexpr ((MODE & kLoss) != 0) {
-        // no block ends while another may still send to it (each of the others has sent, unless a wait ran out)
+        // no block ends while another may still send to it
         __syncwarp();
-        if (p.slices > 1) {
-            asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-            asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-        }
+        if (p.slices > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     }
 }
 
