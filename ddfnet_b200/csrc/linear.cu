@@ -178,8 +178,10 @@ template <typename T, int ACT, bool VEC> __global__ void __launch_bounds__(256) 
                 for (int i = 0; i < 8; ++i) v[i] = Word<T>::get(a[i / 2], i % 2);
                 if constexpr (ACT != kActNone) {
                     const uint32_t b[4] = {z[f].x, z[f].y, z[f].z, z[f].w};
+                    float at[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] *= act_slope<ACT>(Word<T>::get(b[i / 2], i % 2));
+                    for (int i = 0; i < 8; ++i) at[i] = Word<T>::get(b[i / 2], i % 2);
+                    act_slopes<ACT>(v, at);
                     g[f] = make_uint4(Word<T>::put(v[0], v[1]), Word<T>::put(v[2], v[3]), Word<T>::put(v[4], v[5]), Word<T>::put(v[6], v[7]));
                 }
                 if (p.gz) store8(reinterpret_cast<T*>(p.gz) + (r + 8 * f) * p.ldz + col, true, left, g[f]);  // (the workspace's rows)

@@ -47,45 +47,84 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// The normal distribution's Phi(z), and e = exp(-z^2 / 2).  1 - Phi(a) = exp(-a^2 / 2) g(a) for a >= 0, where g falls
-// from 1/2 as 0.4 / a: a polynomial in t = 1 / (1 + 0.315 a) without constant term, fitted for the least relative
-// error over [0, 40] (4.0e-7), by iterated weighted least squares.  erff and expf would cost twice the instructions.
-__device__ __forceinline__ float normal_cdf(float z, float& e) {
-    const float a = fabsf(z), t = __fdividef(1.f, fmaf(0.315f, a, 1.f));
-    float g = 0.034466008f;
-    g = fmaf(g, t, -0.12912883f);
-    g = fmaf(g, t, 0.12538007f);
-    g = fmaf(g, t, 0.0050840266f);
-    g = fmaf(g, t, 0.10151252f);
-    g = fmaf(g, t, 0.1112041f);
-    g = fmaf(g, t, 0.1258197f);
-    g = fmaf(g, t, 0.12566227f);
-    e = exp2_fast(a * a * -0.72134752f);
-    const float q = e * (g * t);
-    return z > 0.f ? 1.f - q : q;
+__device__ __forceinline__ float rcp_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+typedef unsigned long long Pair;  // two floats
+__device__ __forceinline__ Pair both(float v) { return f2_pack(v, v); }
+
+// The normal distribution's Phi(z), and e = exp(-z^2 / 2), of two numbers.  1 - Phi(a) = exp(-a^2 / 2) g(a) for a >= 0,
+// where g falls from 1/2 as 0.4 / a: a polynomial in t = 1 / (1 + 0.315 a) without constant term, fitted for the least
+// relative error over [0, 40] (4.0e-7), by iterated weighted least squares.  12 instructions a number; erff and expf take 40.
+__device__ __forceinline__ Pair normal_cdf(Pair z, Pair& e) {
+    float z0, z1;
+    f2_unpack(z, z0, z1);
+    float d0, d1;
+    f2_unpack(f2_fma(both(0.315f), f2_pack(fabsf(z0), fabsf(z1)), both(1.f)), d0, d1);
+    const Pair t = f2_pack(rcp_fast(d0), rcp_fast(d1));
+    Pair g = both(0.034466008f);
+    g = f2_fma(g, t, both(-0.12912883f));
+    g = f2_fma(g, t, both(0.12538007f));
+    g = f2_fma(g, t, both(0.0050840266f));
+    g = f2_fma(g, t, both(0.10151252f));
+    g = f2_fma(g, t, both(0.1112041f));
+    g = f2_fma(g, t, both(0.1258197f));
+    g = f2_fma(g, t, both(0.12566227f));
+    float h0, h1;
+    f2_unpack(f2_mul(f2_mul(z, z), both(-0.72134752f)), h0, h1);
+    e = f2_pack(exp2_fast(h0), exp2_fast(h1));
+    const Pair q = f2_mul(e, f2_mul(g, t));
+    float q0, q1, p0, p1;
+    f2_unpack(q, q0, q1);
+    f2_unpack(f2_fma(q, both(-1.f), both(1.f)), p0, p1);
+    return f2_pack(z0 > 0.f ? p0 : q0, z1 > 0.f ? p1 : q1);
 }
 template <int ACT> __device__ __forceinline__ float act_value(float z) {
     if constexpr (ACT == kActRelu) return z > 0.f || z != z ? z : 0.f;
-    if constexpr (ACT == kActGelu) {
-        float e;
-        const float phi = normal_cdf(z, e);
-        return z != z ? z : z * phi;
-    }
     if constexpr (ACT == kActSilu) return __fdividef(z, 1.f + exp2_fast(z * -1.4426950f));
+    if constexpr (ACT == kActGelu) {
+        Pair e;
+        float a, b;
+        f2_unpack(normal_cdf(both(z), e), a, b);
+        return z * a;
+    }
     return z;
 }
-template <int ACT> __device__ __forceinline__ float act_slope(float z) {
-    if constexpr (ACT == kActRelu) return z > 0.f ? 1.f : (z != z ? z : 0.f);
-    if constexpr (ACT == kActGelu) {
-        float e;
-        const float phi = normal_cdf(z, e);
-        return z != z ? z : fmaf(z * 0.39894228f, e, phi);
+// act(z) of an even number of values, two at a time.
+template <int ACT, int N> __device__ __forceinline__ void act_values(float (&z)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        if constexpr (ACT == kActGelu) {
+            Pair e;
+            const Pair v = f2_pack(z[i], z[i + 1]);
+            f2_unpack(f2_mul(v, normal_cdf(v, e)), z[i], z[i + 1]);
+        } else {
+            z[i] = act_value<ACT>(z[i]);
+            z[i + 1] = act_value<ACT>(z[i + 1]);
+        }
     }
-    if constexpr (ACT == kActSilu) {
-        const float s = __fdividef(1.f, 1.f + exp2_fast(z * -1.4426950f));
-        return s * (1.f + z * (1.f - s));
+}
+// g *= act'(z)
+template <int ACT, int N> __device__ __forceinline__ void act_slopes(float (&g)[N], const float (&z)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        if constexpr (ACT == kActGelu) {
+            Pair e;
+            const Pair v = f2_pack(z[i], z[i + 1]), phi = normal_cdf(v, e);
+            f2_unpack(f2_mul(f2_pack(g[i], g[i + 1]), f2_fma(f2_mul(v, both(0.39894228f)), e, phi)), g[i], g[i + 1]);
+        } else {
+#pragma unroll
+            for (int j = i; j < i + 2; ++j) {
+                if constexpr (ACT == kActRelu) g[j] = z[j] > 0.f ? g[j] : (z[j] != z[j] ? z[j] : 0.f);
+                if constexpr (ACT == kActSilu) {
+                    const float s = rcp_fast(1.f + exp2_fast(z[j] * -1.4426950f));
+                    g[j] *= s * (1.f + z[j] * (1.f - s));
+                }
+            }
+        }
     }
-    return 1.f;
 }
 __device__ __forceinline__ float act_value(float z, int act) {
     return act == kActRelu ? act_value<kActRelu>(z) : act == kActGelu ? act_value<kActGelu>(z) : act == kActSilu ? act_value<kActSilu>(z) : z;
@@ -274,8 +313,7 @@ __device__ __forceinline__ void finish_piece(const LinearPlan& p, Piece& w, floa
         };
         if (e.residual && !e.after) add();
         if (e.aux) store(&p.aux);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) z[i] = act_value<ACT>(z[i]);
+        act_values<ACT>(z);
         if (e.residual && e.after) add();
         store(&p.y);
         if (e.residual && !own) next();
@@ -290,23 +328,32 @@ __device__ __forceinline__ void finish_piece(const LinearPlan& p, Piece& w, floa
             sts128(w.box + unit64(lane, u), __float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
         }
         __syncwarp();
-        const int in = lane & 15, c = col + 16 * h + in, rows = min(32, p.M - row0);
+        const int in = lane & 15, c = col + 16 * h + in, first = lane >> 4;
         if (c < p.N) {
             const float bias = !p.partial && e.bias ? Elem<T>::load(reinterpret_cast<const T*>(e.bias) + c) : 0.f;
-#pragma unroll 4
-            for (int i = lane >> 4; i < rows; i += 2) {
-                const long long row = row0 + i;
-                float v = ldsf(w.box + unit64(i, in >> 2) + (in & 3) * 4);
-                if (p.partial) {
-                    p.partial[((long long)split * p.M + row) * p.N + c] = v;
-                } else {
-                    const float r = e.residual ? Elem<T>::load(reinterpret_cast<const T*>(e.residual) + row * e.ldr + c) : 0.f;
-                    v += bias;
-                    if (!e.after) v += r;
-                    if (e.aux) Elem<T>::store(reinterpret_cast<T*>(e.aux) + row * e.ldy + c, v);
-                    v = act_value<ACT>(v);
-                    if (e.after) v += r;
-                    Elem<T>::store(reinterpret_cast<T*>(e.y) + row * e.ldy + c, v);
+#pragma unroll
+            for (int eight = 0; eight < 32; eight += 16) {  // eight rows in flight
+                float v[8], r[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = eight + first + 2 * i;
+                    v[i] = ldsf(w.box + unit64(row, in >> 2) + (in & 3) * 4);
+                    r[i] = !p.partial && e.residual && row0 + row < p.M ? Elem<T>::load(reinterpret_cast<const T*>(e.residual) + (long long)(row0 + row) * e.ldr + c) : 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const long long row = row0 + eight + first + 2 * i;
+                    if (row >= p.M) break;
+                    if (p.partial) {
+                        p.partial[((long long)split * p.M + row) * p.N + c] = v[i];
+                        continue;
+                    }
+                    float y = v[i] + bias;
+                    if (!e.after) y += r[i];
+                    if (e.aux) Elem<T>::store(reinterpret_cast<T*>(e.aux) + row * e.ldy + c, y);
+                    y = act_value<ACT>(y);
+                    if (e.after) y += r[i];
+                    Elem<T>::store(reinterpret_cast<T*>(e.y) + row * e.ldy + c, y);
                 }
             }
         }
