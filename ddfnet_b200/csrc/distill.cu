@@ -31,6 +31,7 @@ int device_facts(int* sm_count, int** fault, int* index);
 constexpr int kStats = 8;                     // floats a row between forward and backward
 constexpr int kWarpElements = 1024;           // a row (with what its first granule holds before it) in a warp
 constexpr int kCountBlocks = 128;
+constexpr int kMostDynamic = 200 * 1024;      // bytes of dynamic shared memory
 enum { kLoss = 1, kGrad = 2 };
 
 struct DistillPlan {
@@ -629,7 +630,7 @@ static int distill_launch(DistillPlan p, int sm_count, cudaStream_t st) {
         const size_t granules = (size_t)(per + N - 1) / N + 1;
         const bool resident = granules <= kResidentGranules;
         const size_t bytes = (resident ? granules * 16 : 0) + (MODE & kLoss ? (granules * N + 31) / 32 * 4 : 0);
-        if (bytes > 200 * 1024) return DDF_B200_E_ARGUMENT;
+        if (bytes > kMostDynamic) return DDF_B200_E_ARGUMENT;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(p.rows * slices));
         cfg.blockDim = dim3(kRowThreads);
@@ -645,7 +646,8 @@ static int distill_launch(DistillPlan p, int sm_count, cudaStream_t st) {
         }
         auto kernel = resident ? distill_block_kernel<T, MODE, true> : distill_block_kernel<T, MODE, false>;
         if (bytes > 40 * 1024) {
-            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+            // (the most that any call has: another thread's call may be between this and its launch)
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamic);
             if (e != cudaSuccess) return (int)e;
         }
         const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);

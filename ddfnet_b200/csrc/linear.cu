@@ -267,7 +267,7 @@ static int encode_matrix(CUtensorMap* map, const Matrix& m, int dtype, int box_c
 struct Cut {
     int bn, splits, steps;
 };
-static Cut cut_of(long long M, long long N, long long K, int sm_count) {
+static Cut choose_cut(long long M, long long N, long long K, int sm_count) {
     const long long steps = (K + kTileK - 1) / kTileK, tiles_m = (M + kTileM - 1) / kTileM;
     Cut best{256, 1, (int)steps};
     double least = 1e300;
@@ -289,6 +289,18 @@ static Cut cut_of(long long M, long long N, long long K, int sm_count) {
     }
     return best;
 }
+// A call asks twice or more for the same sizes (scratch, then launch), and the next calls of a program mostly do again.
+static Cut cut_of(long long M, long long N, long long K, int sm_count) {
+    struct Known {
+        long long M, N, K;
+        int sm;
+        Cut cut;
+    };
+    thread_local Known known[16] = {};
+    Known& k = known[(size_t)(M * 7 + N * 3 + K) % 16];
+    if (k.M != M || k.N != N || k.K != K || k.sm != sm_count) k = Known{M, N, K, sm_count, choose_cut(M, N, K, sm_count)};
+    return k.cut;
+}
 static size_t partial_bytes(long long M, long long N, const Cut& c) { return c.splits > 1 ? (size_t)c.splits * M * N * 4 : 0; }
 
 template <typename T, bool AT, bool BT> static auto kernel_of(int bn, int act) {
@@ -298,6 +310,18 @@ template <typename T, bool AT, bool BT> static auto kernel_of(int bn, int act) {
         if (act == kActSilu) return bn == 256 ? linear_kernel<T, 256, AT, BT, kActSilu> : bn == 128 ? linear_kernel<T, 128, AT, BT, kActSilu> : linear_kernel<T, 64, AT, BT, kActSilu>;
     }
     return bn == 256 ? linear_kernel<T, 256, AT, BT, kActNone> : bn == 128 ? linear_kernel<T, 128, AT, BT, kActNone> : linear_kernel<T, 64, AT, BT, kActNone>;
+}
+
+// Lets a kernel have its shared memory: once for each thread, kernel and device, which is also once for each thread's context.
+static int allow_shared(const void* kernel, int device, uint32_t bytes) {
+    thread_local struct { const void* kernel; int device; } done[64] = {};
+    auto& d = done[(reinterpret_cast<uintptr_t>(kernel) >> 4) % 64];
+    if (d.kernel == kernel && d.device == device) return 0;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) return (int)e;
+    d.kernel = kernel;
+    d.device = device;
+    return 0;
 }
 
 // Of a product's waits: their limit, and whether they are made to run out.
@@ -316,9 +340,9 @@ static int product(const Matrix& a, const Matrix& b, long long M, long long N, l
     const Cut cut = cut_of(M, N, K, sm);
     const bool joined = cut.splits > 1;  // by a kernel of its own, which finishes too
     auto kernel = kernel_of<T, AT, BT>(cut.bn, joined ? (int)kActNone : out.act);
-    // (before the driver's encoder: a runtime call gives a thread that has none its context)
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)linear_shared(cut.bn));
-    if (e != cudaSuccess) return (int)e;
+    // (before the driver's encoder: a runtime call that needs the device gives a thread that has none its context)
+    if ((rc = allow_shared((const void*)kernel, index, linear_shared(cut.bn)))) return rc;
+    cudaError_t e;
     LinearPlan p{};
     if ((rc = encode_matrix(&p.a, a, dtype, 64, AT ? kTileK : kTileM))) return rc;
     if ((rc = encode_matrix(&p.b, b, dtype, 64, BT ? kTileK : cut.bn))) return rc;

@@ -375,7 +375,7 @@ static int top_launch(const TopPlan& p, long long rows, cudaStream_t st) {
     const size_t bytes = ((size_t)p.V * sizeof(T) + 15) / 16 * 16 + 16;  // a granule more for a row that starts inside one
     if (bytes <= (size_t)kResidentGranules * 16) {
         if (bytes > 36 * 1024) {  // with the static part beyond what a block gets unasked
-            const cudaError_t e = cudaFuncSetAttribute(top_logits_kernel<T, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+            const cudaError_t e = cudaFuncSetAttribute(top_logits_kernel<T, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kResidentGranules * 16);
             if (e != cudaSuccess) return (int)e;
         }
         top_logits_kernel<T, NT, true><<<(unsigned)rows, NT, bytes, st>>>(p);
