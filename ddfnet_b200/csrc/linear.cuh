@@ -468,17 +468,27 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
         const bool residual = p.out.residual && p.boxes && !p.partial;
         const uint32_t box = pieces + (uint32_t)(warp - 4) * kBoxes * kBox;
         Piece w{box, res_bar(warp - 4), residual ? 1 : kBoxes, 0, box + (kBoxes - 1) * kBox, 0u, false};
-        // the residual's copy runs one piece ahead
-        int fetch_item = blockIdx.x, fetch_c = c0, fetch_m = 0, fetch_n = 0, unused;
-        if (residual && fetch_item < items) tile_of(p, fetch_item, fetch_m, fetch_n, unused);
+        // the residual's copy runs one piece ahead, and another tile ahead of that its way into the second-level cache
+        int fetch_item = blockIdx.x, fetch_c = c0, fetch_m = 0, fetch_n = 0, ahead_m = 0, ahead_n = 0, unused;
+        const auto look_ahead = [&] {
+            if (fetch_item + (int)gridDim.x < items) tile_of(p, fetch_item + gridDim.x, ahead_m, ahead_n, unused);
+        };
+        if (residual && fetch_item < items) {
+            tile_of(p, fetch_item, fetch_m, fetch_n, unused);
+            look_ahead();
+        }
         const auto next = [&] {
             if (fetch_item >= items) return;
             fetch_residual(p, w, fetch_m * kTileM + quarter * 32, fetch_n * BN + fetch_c, lane);
+            if (lane == 0 && fetch_item + (int)gridDim.x < items)
+                tma_prefetch_2d(&p.r, ahead_n * BN + fetch_c, ahead_m * kTileM + quarter * 32);
             fetch_c += 32;
             if (fetch_c == c1) {
                 fetch_c = c0;
                 fetch_item += gridDim.x;
-                if (fetch_item < items) tile_of(p, fetch_item, fetch_m, fetch_n, unused);
+                fetch_m = ahead_m;
+                fetch_n = ahead_n;
+                look_ahead();
             }
         };
         if (residual) next();
