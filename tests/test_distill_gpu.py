@@ -91,7 +91,8 @@ def check_loss(got, want, t):
 
 # ------------------------------------------------------------------ top logits
 SIZES = [(1, 1, 1), (3, 2, 2), (2, 7, 3), (5, 31, 31), (4, 100, 20), (9, 1000, 20), (3, 1009, 128), (2, 1025, 129),
-         (2, 4099, 256), (3, 32003, 64), (1, 65536, 40), (2, 131075, 33), (160, 40000, 17)]
+         (2, 4099, 256), (3, 32003, 64), (1, 65536, 40), (2, 131075, 33), (160, 40000, 17), (11, 474, 111), (69, 1000, 116), (40, 1000, 256),
+         (160, 8000, 200)]
 
 
 @pytest.mark.parametrize("dt", list(DTYPES))
