@@ -19,7 +19,7 @@
 // them out of each other's shared memory gained at most half a microsecond where all its blocks fit at once, and lost
 // eight where they did not.)
 //
-// Measured (in a graph): 8192x2048x8192 bfloat16 189 us (1.45 PFLOP/s, nine tenths of the library's burst rate), with bias and GELU
+// Measured (in a graph): 8192x2048x8192 bfloat16 189 us (1.45 PFLOP/s under the power cap, 168 us before it bites), with bias and GELU
 // 202; 100352x128x512 float16 24.4 us (5.3 TB/s), with bias, residual and ReLU 43; 32x4096x4096 10.1.
 //
 // Every wait is bounded: a role whose wait runs out records a fault and leaves its loop, the others follow by their

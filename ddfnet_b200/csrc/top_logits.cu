@@ -16,8 +16,8 @@
 //      Their elements then get a thread each, and go to the sum or to the list of elements.
 //   3. Each listed element counts the elements ahead of it, by one 64-bit key (value, then lower class first):
 //      its place, or, past k, one more summand of the rest.
-// Measured: 4096 rows of 32768 bfloat16 logits, k = 64, 109 us (2.5 TB/s; 3.7 instructions a clock and SM, where the bytes alone
-// would take 41); 256 rows of 1000 float16, k = 20, 5.7 in a graph.  512 threads a row: 100 us before the lists had an order, 256
+// Measured: 4096 rows of 32768 bfloat16 logits, k = 64, 109 us (2.5 TB/s, 78 % of the issue slots busy, where the bytes
+// alone would take 41); 256 rows of 1000 float16, k = 20, 5.7 in a graph.  512 threads a row: 100 us before the lists had an order, 256
 // threads 111.
 // A list that runs over (rows of few distinct values, masked rows) takes the general way instead: a
 // radix selection of the k-th key over four histograms, then one ordered pass that fills in its equals.
