@@ -494,10 +494,10 @@ static int backward(const ddf_b200_linear_args* q, const void* gy, long long gy_
     Matrix gz{as_gy ? gy : as_gr ? gr : nullptr, M, N, as_gy ? gy_stride : as_gr ? N : padded(N)};
     void* gzp = scratch ? ws.take((size_t)M * padded(N) * 2) : nullptr;
     if (scratch) gz.p = gzp;
-    // rows of a block: four blocks an SM, 512 sums a column at most
+    // rows of a block: four blocks an SM, 512 sums a column at most; a warp has four rows in flight
     long long chunk = M * ((N + 255) / 256) / (4 * sm);
     chunk = chunk < (M + 511) / 512 ? (M + 511) / 512 : chunk;
-    chunk = (chunk + 8) / 8 * 8;
+    chunk = chunk < 32 ? 32 : (chunk + 7) / 8 * 8;
     const long long chunks = (M + chunk - 1) / chunk;
     float* sums = gb ? (float*)ws.take((size_t)chunks * N * 4) : nullptr;
     Matrix x{q->x, M, K, q->x_stride}, w{q->weight, N, K, q->weight_stride};
